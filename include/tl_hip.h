@@ -204,6 +204,109 @@ int tl_hip_launch_quant_gemm_noalloc(const tl_hip_qtensor* w, const float* x, fl
  * parity tests (which kernel variant ran); no reference counterpart. */
 int tl_hip_debug_last_gemm_plan(int* tile_m, int* tile_n, int* k_splits);
 
+/* ------------------------------------------------------------- paged KV cache ---- */
+/* Keys and values of several sequences in pages of page_size positions, and the attention that
+ * reads them (no reference counterpart: KVCache, system.rs:387-600, holds one dense sequence).
+ * Launchers on device pointers, as the quantized ones above.
+ *
+ *   k_pages, v_pages  [n_pages, n_kv_heads, page_size, head_dim], kv_dtype TL_HIP_F16 or TL_HIP_F32;
+ *                     page_size a power of two from 16 to 32768, head_dim a multiple of 8 up to 256
+ *   page_table        int32 [batch, table_stride]: position j of sequence b lies in page
+ *                     page_table[b][j / page_size] at slot j % page_size
+ *   kv_lens           int32 [batch]: positions of each sequence, the new ones included
+ *   cu_seqlens        int32 [batch + 1], not falling: the packed rows cu_seqlens[b] ..
+ *                     cu_seqlens[b + 1] - 1 of n_tokens rows are sequence b's new positions, the
+ *                     last of its kv_lens[b].  Rows from cu_seqlens[batch] on belong to no
+ *                     sequence: they are not read, and rows of out are left as they were.
+ *
+ * The integer arrays are device memory and read by the kernels (a captured call follows their
+ * current values at each replay); what they may hold is checked there, never followed out of
+ * range: values of cu_seqlens outside 0 .. n_tokens and kv_lens outside 0 .. table_stride *
+ * page_size are taken as the nearest bound.  A table entry outside 0 .. n_pages - 1 makes the
+ * attention rows that see its positions NaN, and appends nothing; so does a kv_lens past the
+ * table's positions for the rows at positions past them.  Entries past a sequence's length are
+ * not read.
+ * Pointers to keys, values, queries and rows are 16-byte aligned, and row strides (in elements)
+ * multiples of 16 bytes (ArgumentError otherwise).  stream NULL = the library's.  Sequences are
+ * independent: two calls overlap on different streams as long as neither writes what the other
+ * reads.
+ *
+ * tl_hip_launch_kv_append writes row t's keys and values (k_new + t * k_row_stride, n_kv_heads *
+ * head_dim of new_dtype F32 or F16; likewise v_new) to its position's slot, rounded to nearest
+ * where the cache is f16.  No other byte of the pages changes.  Rows whose position is below 0
+ * (more new rows than kv_lens) are dropped. */
+int tl_hip_launch_kv_append(const void* k_new, const void* v_new, int new_dtype, int64_t k_row_stride,
+                            int64_t v_row_stride, void* k_pages, void* v_pages, int kv_dtype, int64_t n_pages,
+                            int page_size, int n_kv_heads, int head_dim, const int32_t* page_table,
+                            int64_t table_stride, const int32_t* cu_seqlens, const int32_t* kv_lens, int64_t batch,
+                            int64_t n_tokens, void* stream);
+/* Copies page src[i] to page dst[i], i < n_pairs, in K and V of every layer: pools k_pages and
+ * v_pages [n_layers, n_pages, page_bytes], page_bytes a multiple of 16.  src and dst are host
+ * memory, read before the call returns (under capture the pairs are part of the graph).
+ * Sources may repeat; destinations may not, and none may be a source (ArgumentError), so that the
+ * order of the copies does not matter; page numbers outside the pool are IndexOutOfBounds. */
+int tl_hip_launch_kv_copy_pages(void* k_pages, void* v_pages, int64_t n_layers, int64_t n_pages, int64_t page_bytes,
+                                const int32_t* src, const int32_t* dst, int64_t n_pairs, void* stream);
+/* Attention of one new token per sequence: q [batch, n_heads, head_dim] (row b at q + b *
+ * q_row_stride), out [batch, n_heads, head_dim] of q's type;
+ *   out[b][h] = sum_j softmax_j(scale q[b][h] . k_j) v_j over the kv_lens[b] positions j,
+ * query head h reading KV head h / (n_heads / n_kv_heads); zeros for a sequence of length 0.
+ * Types (q_dtype, kv_dtype): (F32, F32) and (F32, F16), f32 arithmetic and results within the f32
+ * class; (F16, F16), results rounded to f16 once.
+ * workspace: at least tl_hip_paged_attention_workspace(...) bytes of device memory, 16-byte
+ * aligned and used by one call at a time, or NULL: the library's allocator then lends it (refused
+ * under stream capture, ArgumentError: a graph keeps its workspace, so the caller has to own it). */
+int tl_hip_launch_paged_attention_decode(const void* q, int q_dtype, int64_t q_row_stride, const void* k_pages,
+                                         const void* v_pages, int kv_dtype, int64_t n_pages, int page_size,
+                                         int n_heads, int n_kv_heads, int head_dim, const int32_t* page_table,
+                                         int64_t table_stride, const int32_t* kv_lens, int64_t batch, void* out,
+                                         float scale, void* workspace, size_t workspace_bytes, void* stream);
+/* Causal attention of packed rows, prompts or later chunks of them: the rows of sequence b (n_b =
+ * cu_seqlens[b + 1] - cu_seqlens[b]) are queries at positions kv_lens[b] - n_b + i, each over the
+ * positions up to its own.  q [n_tokens, n_heads, head_dim], out alike; a row at a position below
+ * 0 sees nothing and is zeros.  Keys and values of the new positions are appended before the call.
+ * An infinite or NaN value at a position reaches only the rows that see it, which become infinite
+ * or NaN in that dimension.  The rest as tl_hip_launch_paged_attention_decode; (F16, F16) rounds
+ * the softmax weights to f16 on the way. */
+int tl_hip_launch_paged_attention_prefill(const void* q, int q_dtype, int64_t q_row_stride, const void* k_pages,
+                                          const void* v_pages, int kv_dtype, int64_t n_pages, int page_size,
+                                          int n_heads, int n_kv_heads, int head_dim, const int32_t* page_table,
+                                          int64_t table_stride, const int32_t* cu_seqlens, const int32_t* kv_lens,
+                                          int64_t batch, int64_t n_tokens, void* out, float scale, void* workspace,
+                                          size_t workspace_bytes, void* stream);
+/* Workspace bytes of both (n_tokens = batch for decode), whatever the lengths; 0 + ArgumentError
+ * for sizes that the launchers refuse. */
+size_t tl_hip_paged_attention_workspace(int64_t batch, int64_t n_tokens, int n_heads, int n_kv_heads, int head_dim);
+
+/* The host's book of such a cache: which pages each sequence holds and how many share a page.
+ * Host memory only; one thread at a time per book.  The book decides, the caller acts: it copies
+ * the (src, dst) pairs that a call returns with tl_hip_launch_kv_copy_pages before anything writes
+ * the pages again, and uploads the table rows.  Page choices are the lowest free pages, always.
+ * A book is a handle from tl_hip_page_book_new (NULL + error otherwise). */
+void* tl_hip_page_book_new(int64_t n_pages, int page_size);
+int tl_hip_page_book_release(void* book);
+/* A new empty sequence, and one that shares all pages of `seq`; the id (>= 0), -1 on error. */
+int64_t tl_hip_page_book_open(void* book);
+int64_t tl_hip_page_book_fork(void* book, int64_t seq);
+/* Ends a sequence: pages that no other sequence holds are free again. */
+int tl_hip_page_book_close(void* book, int64_t seq);
+/* Room for n_tokens more positions.  A shared tail page that would be written is replaced by a
+ * page of the sequence's own: the pair goes to src[0], dst[0] and *n_pairs is 1, else 0.
+ * AllocationError, with nothing changed, when too few pages are free. */
+int tl_hip_page_book_grow(void* book, int64_t seq, int64_t n_tokens, int32_t* src, int32_t* dst, int64_t* n_pairs);
+/* Drops the positions from `length` on (rejected drafts, an edited chat). */
+int tl_hip_page_book_cut(void* book, int64_t seq, int64_t length);
+/* Moves the used pages down to pages 0 .. used - 1.  src and dst hold `capacity` pairs; with less
+ * room than *n_pairs (at most the number of used pages) nothing changes and the call is
+ * ArgumentError. */
+int tl_hip_page_book_compact(void* book, int32_t* src, int32_t* dst, int64_t capacity, int64_t* n_pairs);
+/* Positions of a sequence and free pages of the book (-1 on error). */
+int64_t tl_hip_page_book_length(const void* book, int64_t seq);
+int64_t tl_hip_page_book_free_pages(const void* book);
+/* The sequence's row of the page table: its pages, then -1 up to `capacity` entries
+ * (ArgumentError when it holds more pages). */
+int tl_hip_page_book_row(const void* book, int64_t seq, int32_t* row, int64_t capacity);
+
 /* ------------------------------------------------------------ tensor operators --- */
 /* IDevice::tensor_matmul (device.rs:258; tl_cpu tensor.rs:1248-1313): [.., m, k] x
  * [.., k, n] (b batched only when its rank > 2) or 1-D operands. */

@@ -156,6 +156,115 @@ extern "C" {
         tile_n: *mut i32,
         k_splits: *mut i32,
     ) -> i32;
+    pub fn tl_hip_launch_kv_append(
+        k_new: *const c_void,
+        v_new: *const c_void,
+        new_dtype: i32,
+        k_row_stride: i64,
+        v_row_stride: i64,
+        k_pages: *mut c_void,
+        v_pages: *mut c_void,
+        kv_dtype: i32,
+        n_pages: i64,
+        page_size: i32,
+        n_kv_heads: i32,
+        head_dim: i32,
+        page_table: *const i32,
+        table_stride: i64,
+        cu_seqlens: *const i32,
+        kv_lens: *const i32,
+        batch: i64,
+        n_tokens: i64,
+        stream: *mut c_void,
+    ) -> i32;
+    pub fn tl_hip_launch_kv_copy_pages(
+        k_pages: *mut c_void,
+        v_pages: *mut c_void,
+        n_layers: i64,
+        n_pages: i64,
+        page_bytes: i64,
+        src: *const i32,
+        dst: *const i32,
+        n_pairs: i64,
+        stream: *mut c_void,
+    ) -> i32;
+    pub fn tl_hip_launch_paged_attention_decode(
+        q: *const c_void,
+        q_dtype: i32,
+        q_row_stride: i64,
+        k_pages: *const c_void,
+        v_pages: *const c_void,
+        kv_dtype: i32,
+        n_pages: i64,
+        page_size: i32,
+        n_heads: i32,
+        n_kv_heads: i32,
+        head_dim: i32,
+        page_table: *const i32,
+        table_stride: i64,
+        kv_lens: *const i32,
+        batch: i64,
+        out: *mut c_void,
+        scale: f32,
+        workspace: *mut c_void,
+        workspace_bytes: usize,
+        stream: *mut c_void,
+    ) -> i32;
+    pub fn tl_hip_launch_paged_attention_prefill(
+        q: *const c_void,
+        q_dtype: i32,
+        q_row_stride: i64,
+        k_pages: *const c_void,
+        v_pages: *const c_void,
+        kv_dtype: i32,
+        n_pages: i64,
+        page_size: i32,
+        n_heads: i32,
+        n_kv_heads: i32,
+        head_dim: i32,
+        page_table: *const i32,
+        table_stride: i64,
+        cu_seqlens: *const i32,
+        kv_lens: *const i32,
+        batch: i64,
+        n_tokens: i64,
+        out: *mut c_void,
+        scale: f32,
+        workspace: *mut c_void,
+        workspace_bytes: usize,
+        stream: *mut c_void,
+    ) -> i32;
+    pub fn tl_hip_paged_attention_workspace(
+        batch: i64,
+        n_tokens: i64,
+        n_heads: i32,
+        n_kv_heads: i32,
+        head_dim: i32,
+    ) -> usize;
+    pub fn tl_hip_page_book_new(n_pages: i64, page_size: i32) -> *mut c_void;
+    pub fn tl_hip_page_book_release(book: *mut c_void) -> i32;
+    pub fn tl_hip_page_book_open(book: *mut c_void) -> i64;
+    pub fn tl_hip_page_book_fork(book: *mut c_void, seq: i64) -> i64;
+    pub fn tl_hip_page_book_close(book: *mut c_void, seq: i64) -> i32;
+    pub fn tl_hip_page_book_grow(
+        book: *mut c_void,
+        seq: i64,
+        n_tokens: i64,
+        src: *mut i32,
+        dst: *mut i32,
+        n_pairs: *mut i64,
+    ) -> i32;
+    pub fn tl_hip_page_book_cut(book: *mut c_void, seq: i64, length: i64) -> i32;
+    pub fn tl_hip_page_book_compact(
+        book: *mut c_void,
+        src: *mut i32,
+        dst: *mut i32,
+        capacity: i64,
+        n_pairs: *mut i64,
+    ) -> i32;
+    pub fn tl_hip_page_book_length(book: *const c_void, seq: i64) -> i64;
+    pub fn tl_hip_page_book_free_pages(book: *const c_void) -> i64;
+    pub fn tl_hip_page_book_row(book: *const c_void, seq: i64, row: *mut i32, capacity: i64) -> i32;
     pub fn tl_hip_tensor_matmul(
         a: *const tl_hip_tensor,
         b: *const tl_hip_tensor,

@@ -71,6 +71,22 @@ PROTOS = {
     "tl_hip_launch_quant_gemm_noalloc": (i32, [P, P, P, i64, i32, P]),
     "tl_hip_read_floor": (i32, [P, P]),
     "tl_hip_debug_last_gemm_plan": (i32, [i32p, i32p, i32p]),
+    "tl_hip_launch_kv_append": (i32, [P, P, i32, i64, i64, P, P, i32, i64, i32, i32, i32, P, i64, P, P, i64, i64, P]),
+    "tl_hip_launch_kv_copy_pages": (i32, [P, P, i64, i64, i64, i32p, i32p, i64, P]),
+    "tl_hip_launch_paged_attention_decode": (i32, [P, i32, i64, P, P, i32, i64, i32, i32, i32, i32, P, i64, P, i64, P, f32, P, sz, P]),
+    "tl_hip_launch_paged_attention_prefill": (i32, [P, i32, i64, P, P, i32, i64, i32, i32, i32, i32, P, i64, P, P, i64, i64, P, f32, P, sz, P]),
+    "tl_hip_paged_attention_workspace": (sz, [i64, i64, i32, i32, i32]),
+    "tl_hip_page_book_new": (P, [i64, i32]),
+    "tl_hip_page_book_release": (i32, [P]),
+    "tl_hip_page_book_open": (i64, [P]),
+    "tl_hip_page_book_fork": (i64, [P, i64]),
+    "tl_hip_page_book_close": (i32, [P, i64]),
+    "tl_hip_page_book_grow": (i32, [P, i64, i64, i32p, i32p, i64p]),
+    "tl_hip_page_book_cut": (i32, [P, i64, i64]),
+    "tl_hip_page_book_compact": (i32, [P, i32p, i32p, i64, i64p]),
+    "tl_hip_page_book_length": (i64, [P, i64]),
+    "tl_hip_page_book_free_pages": (i64, [P]),
+    "tl_hip_page_book_row": (i32, [P, i64, i32p, i64]),
     "tl_hip_tensor_matmul": (P, [P, P]),
     "tl_hip_tensor_transpose_2d": (P, [P]),
     "tl_hip_tensor_transpose": (P, [P, i64, i64]),

@@ -63,6 +63,10 @@ class HipTensor:
         return int(self._lib.tl_hip_tensor_numel(self._h))
 
     @property
+    def dtype(self):
+        return int(self._lib.tl_hip_tensor_dtype(self._h))
+
+    @property
     def data_ptr(self):
         return self._lib.tl_hip_tensor_data(self._h)
 
