@@ -1,63 +1,599 @@
-// Attention over a paged KV cache: one wavefront per (row, head), the general form.
+// Attention over a paged KV cache, for one new token per sequence and for packed rows.
+//
+// Rows: the (query, head) pairs of a sequence that share a KV head, 16 to a tile.  With scores
+// s_j = q . k_j, c = scale log2(e) and a running maximum m of the scores seen, one pass keeps
+//   l = sum_j 2^(c (s_j - m)),  o = sum_j 2^(c (s_j - m)) v_j,
+// both multiplied by 2^(c (m_old - m_new)) where the maximum rises; out = o / l.  Parts of the
+// positions join the same way.
 #include "paged.h"
+
+#include <cfloat>
+#include <type_traits>
 
 namespace tlhip {
 
-template <typename QT, typename KVT>
-__global__ __launch_bounds__(64) void k_paged_rows(const PagedAttn a) {
-    const PagedCache& c = a.c;
-    const int lane = threadIdx.x, t = blockIdx.x / a.hq, h = blockIdx.x % a.hq;
-    int b = 0, first = 0, n = 0;
-    for (; b < c.batch; b++) {
-        n = paged_rows(c, b, &first);
-        if (t >= first && t < first + n) break;
-    }
-    if (b == c.batch) return;
+typedef _Float16 half4v __attribute__((ext_vector_type(4)));
+
+// ---- which work is whose ---------------------------------------------------------------
+// k_paged_tile: sequence b has tiles(b) row tiles per KV head and rounds(b) rounds of KEYS
+// positions; the call's work is the line of all (sequence, KV head, tile, round) in that order,
+// cut into equal runs, one per workgroup, whatever the lengths.  A tile whose rounds lie in one
+// run is finished there; otherwise each run leaves a record (o, m, c, l of 16 rows) in the
+// workspace: the run that begins the tile in its slot 1, the others in slot 0, and k_paged_join
+// adds them in order.
+constexpr int RUNS = 512;  // at most: two workgroups per CU
+
+struct Work {
+    int tiles, rounds;
+};
+__device__ __forceinline__ Work work_of(const PagedCache& c, int b, int G, int keys) {
     bool past;
-    const int len = paged_len(c, b, &past);
-    const int64_t want = (int64_t)max(c.lens[b], 0) - n + (t - first) + 1;  // positions this row sees
-    const int limit = (int)min(want, (int64_t)len);
-    const int G = a.hq / c.hkv, page = 1 << c.shift;
-    const QT* q = static_cast<const QT*>(a.q) + t * a.q_stride + h * c.D;
-    float qv[4], o[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
+    int first;
+    const int n = paged_rows(c, b, &first);
+    if (n == 0) return {0, 0};
+    return {(n * G + 15) >> 4, (paged_len(c, b, &past) + keys - 1) / keys};
+}
+__device__ __forceinline__ int64_t lane_value(int64_t v, int lane) {
+    return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)v, lane) |
+                     (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32);
+}
+// sum over lanes 0 .. this one
+__device__ __forceinline__ int64_t lane_prefix(int64_t v) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) qv[i] = lane + 64 * i < c.D ? (float)q[lane + 64 * i] * (a.scale * 1.44269504088896341f) : 0.f;
-    for (int j = 0; j < limit; j++) {
-        const int p = c.table[b * c.table_stride + (j >> c.shift)];
-        const bool bad = (uint32_t)p >= (uint32_t)c.n_pages;
-        const int64_t at = (bad ? 0 : p) * c.page_elems + ((int64_t)(h / G) * page + (j & (page - 1))) * c.D;
-        float x = 0.f, v[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const bool in = lane + 64 * i < c.D;
-            x = fmaf(qv[i], in ? (float)static_cast<const KVT*>(c.k)[at + lane + 64 * i] : 0.f, x);
-            v[i] = in ? (float)static_cast<const KVT*>(c.v)[at + lane + 64 * i] : 0.f;
-        }
-        x = wave_allsum(x);
-        if (bad) x = NAN;
-        const float mn = fmaxf(m, x), ms = mn == -INFINITY ? 0.f : mn;
-        const float al = __builtin_amdgcn_exp2f(m - ms), e = __builtin_amdgcn_exp2f(x - ms);
-        m = mn;
-        l = fmaf(l, al, e);
-#pragma unroll
-        for (int i = 0; i < 4; i++) o[i] = fmaf(o[i], al, e * v[i]);
+    for (int off = 1; off < 64; off <<= 1) {
+        const int64_t o = __shfl_up(v, off);
+        if ((int)__lane_id() >= off) v += o;
     }
-    const float inv = limit < want ? NAN : 1.0f / l;
-    QT* op = static_cast<QT*>(a.out) + ((int64_t)t * a.hq + h) * c.D;
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-        if (lane + 64 * i < c.D) op[lane + 64 * i] = (QT)(want <= 0 ? 0.f : o[i] * inv);
+    return v;
+}
+__device__ __forceinline__ uint32_t div_u(int64_t a, int64_t b) {
+    if (((a | b) >> 32) == 0) return (uint32_t)a / (uint32_t)b;
+    return (uint32_t)((uint64_t)a / (uint64_t)b);
 }
 
-size_t paged_attention_workspace(int64_t batch, int64_t rows, int hq, int hkv, int D) { return 16; }
+// All ones over the f32 or the two f16 of a word that are infinite or NaN, else 0.
+template <typename T>
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+    if constexpr (sizeof(T) == 4) return (uint32_t)((int32_t)((w & 0x7F800000u) + 0x00800000u) >> 31);
+    const uint32_t top = ((w & 0x7C007C00u) + 0x04000400u) & 0x80008000u;  // the exponent's carry
+    return (top - (top >> 15)) | top;
+}
 
-int launch_paged_attention(const PagedAttn& a, bool q16, bool kv16, hipStream_t s) {
-    const dim3 grid((unsigned)((int64_t)a.c.rows * a.hq));
-    if (q16) k_paged_rows<_Float16, _Float16><<<grid, 64, 0, s>>>(a);
-    else if (kv16) k_paged_rows<float, _Float16><<<grid, 64, 0, s>>>(a);
-    else k_paged_rows<float, float><<<grid, 64, 0, s>>>(a);
+// ---- 16 rows, keys and values straight from memory into matrix operands ------------------
+// A wavefront takes 16 TK positions of a round at a time, the four wavefronts of a workgroup
+// the four parts of a round; they add up in LDS at the end of a tile's run.
+//   S^T = K Q^T: lane (col, g) = (l % 16, l / 16) holds 16-byte pieces of key 16 t + col, the
+//     operand A of the matrix instruction as they stand, and gets the scores of row col at keys
+//     16 t + 4 g + e;
+//   O^T += V^T P^T with those keys as its k slots, so P stays where the scores are.  The lane
+//     loads 4 TK keys' values at the same few dimensions (VE of them, 16 lanes together a
+//     whole row): the operand for dimension x of these takes element x of each, and row r of the
+//     product is dimension VE r + x.
+// f16 caches: products exact in f32; f32 rows enter as two f16 parts (row scaled by a power of
+// two, 22 bits), weights as two parts of 2^15 p, so the results keep f32's digits.  f32 caches:
+// f32 matrix instructions.
+template <typename KVT, typename QT, int DP, int TK>
+struct Tile {
+    static constexpr bool H16 = std::is_same_v<KVT, _Float16>;
+    static constexpr int QP = H16 && std::is_same_v<QT, float> ? 2 : 1;  // parts of a query
+    static constexpr int PIECE = 16 / sizeof(KVT);                       // elements per 16 bytes
+    static constexpr int KS = DP / (4 * PIECE);                          // pieces of a key per lane
+    static constexpr int VE = DP / 16 < PIECE ? DP / 16 : PIECE;         // value elements per load
+    static constexpr int VN = DP / 16 / VE;                              // loads per value row and lane
+    static constexpr int NA = DP / 16;
+    static constexpr int KEYS = 64 * TK;  // positions per round
+};
+
+// FULL: head_dim is DP (otherwise the rest of a key's pieces are zeros; the rest of a value's
+// make rows of the product that are not stored, and read the row's first elements).
+template <typename KVT, typename QT, int DP, int TK, bool FULL>
+__global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_tile(
+    const PagedAttn a, const int32_t* __restrict__ table, const char* __restrict__ kp, const char* __restrict__ vp) {
+    using L = Tile<KVT, QT, DP, TK>;
+    constexpr int QP = L::QP, KS = L::KS, VE = L::VE, VN = L::VN, NA = L::NA, KEYS = L::KEYS, EB = sizeof(KVT);
+    constexpr bool H16 = L::H16;
+    typedef KVT vec __attribute__((ext_vector_type(VE)));
+    typedef uint32_t words __attribute__((ext_vector_type(sizeof(vec) / 4)));
+    typedef KVT piece __attribute__((ext_vector_type(L::PIECE)));
+    constexpr int RS = DP + 4;
+    __shared__ __attribute__((aligned(16))) float so[4][16][RS];  // o, then m and l
+    const PagedCache& c = a.c;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
+    const int G = a.G, D = FULL ? DP : c.D, page = 1 << c.shift;
+    // run: neighbours on the line stay on one XCD (workgroups go round the eight of them)
+    const int runs = gridDim.x, id = blockIdx.x;
+    const int run = (runs & 7) == 0 ? (id & 7) * (runs >> 3) + (id >> 3) : id;
+
+    int64_t total = 0, incl = 0, mine = 0;
+    for (int base = 0; base < c.batch; base += 64) {
+        Work w{0, 0};
+        if (base + lane < c.batch) w = work_of(c, base + lane, G, KEYS);
+        mine = (int64_t)c.hkv * w.tiles * w.rounds;
+        incl = lane_prefix(mine);
+        total += lane_value(incl, 63);
+    }
+    const int64_t len_run = total <= runs ? 1 : total <= 0x7FFFFFFF ? ((uint32_t)total + runs - 1) / (uint32_t)runs : (total + runs - 1) / runs;
+    int64_t x = run * len_run;
+    const int64_t x1 = min(x + len_run, total);
+    if (x >= x1) return;
+    int b = 0;
+    int64_t before = 0;  // line position of sequence b's first round
+    for (int base = 0;; base += 64) {
+        if (c.batch > 64) {
+            Work w{0, 0};
+            if (base + lane < c.batch) w = work_of(c, base + lane, G, KEYS);
+            mine = (int64_t)c.hkv * w.tiles * w.rounds;
+            incl = lane_prefix(mine);
+        }
+        const uint64_t hit = __ballot(x < before + incl);
+        if (hit) {
+            const int at = __builtin_ctzll(hit);
+            b = base + at;
+            before += lane_value(incl, at) - lane_value(mine, at);
+            break;
+        }
+        before += lane_value(incl, 63);
+    }
+    b = __builtin_amdgcn_readfirstlane(b);
+
+    while (x < x1) {
+        const Work w = work_of(c, b, G, KEYS);
+        const int64_t here = (int64_t)c.hkv * w.tiles * w.rounds;
+        if (x >= before + here) {
+            before += here;
+            b++;
+            continue;
+        }
+        const uint32_t unit = __builtin_amdgcn_readfirstlane(div_u(x - before, w.rounds));
+        const int r0 = __builtin_amdgcn_readfirstlane((int)(x - before - (int64_t)unit * w.rounds));
+        const int r1 = __builtin_amdgcn_readfirstlane((int)min((int64_t)w.rounds, r0 + (x1 - x)));
+        const int h = unit / w.tiles, tile = unit - h * w.tiles;
+        x += r1 - r0;
+
+        // this lane's row
+        int first;
+        bool past;
+        const int n = paged_rows(c, b, &first), len = paged_len(c, b, &past), rows = n * G;
+        const int64_t shown = (int64_t)max(c.lens[b], 0) - n + 1;  // positions that query 0 sees
+        const int r = min(tile * 16 + col, rows - 1), qi = r / G, qh = h * G + r - qi * G;
+        const int lim = (int)max(min(shown + qi, (int64_t)len), (int64_t)0);
+        const int lim_lo = (int)max(min(shown + tile * 16 / G, (int64_t)len), (int64_t)0);
+        const int lim_hi = (int)max(min(shown + min(tile * 16 + 15, rows - 1) / G, (int64_t)len), (int64_t)0);
+
+        const QT* qp = static_cast<const QT*>(a.q) + (int64_t)(first + qi) * a.q_stride + qh * D;
+        float cs = fminf(fabsf(a.scale) * 1.44269504088896341f, FLT_MAX);
+        const float sign = a.scale < 0.f ? -1.f : a.scale > 0.f ? 1.f : 0.f;
+        typedef std::conditional_t<H16, half8, floatx4> qvec;
+        qvec qf[QP][KS];
+        if constexpr (H16) {
+            float qv[KS][8];
+            float top = 0.f;
+#pragma unroll
+            for (int s = 0; s < KS; s++) {
+                const bool in = 32 * s + 8 * g < D;
+                if constexpr (QP == 2) {
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const floatx4 f = in ? reinterpret_cast<const floatx4*>(qp + 32 * s + 8 * g)[e] : floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int i = 0; i < 4; i++) qv[s][4 * e + i] = f[i] * sign, top = fmaxf(top, fabsf(f[i]));
+                    }
+                } else {
+                    half8 z = {};
+                    if (in) z = *reinterpret_cast<const half8*>(qp + 32 * s + 8 * g);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) qf[0][s][i] = z[i] * (_Float16)sign;
+                }
+            }
+            if constexpr (QP == 2) {
+                top = lane_pair_max<16>(top);
+                top = lane_pair_max<32>(top);
+                // the row's largest entry to 2^14 .. 2^15
+                const int up = top > 0.f && top <= FLT_MAX ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
+                cs = fminf(ldexpf(fabsf(a.scale) * 1.44269504088896341f, -up), FLT_MAX);
+#pragma unroll
+                for (int s = 0; s < KS; s++)
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const float f = ldexpf(qv[s][i], up);
+                        qf[0][s][i] = (_Float16)f;
+                        qf[1][s][i] = (_Float16)(f - (float)qf[0][s][i]);
+                    }
+            }
+        } else {
+#pragma unroll
+            for (int s = 0; s < KS; s++) {
+                floatx4 f = {};
+                if (16 * s + 4 * g < D) f = *reinterpret_cast<const floatx4*>(qp + 16 * s + 4 * g);
+#pragma unroll
+                for (int i = 0; i < 4; i++) qf[0][s][i] = f[i] * sign;
+            }
+        }
+        cs = fmaxf(cs, FLT_MIN);
+
+        // positions of this wavefront: blocks of 16 TK from j_of(0), every KEYS
+        const int64_t head = (int64_t)h * page * D * EB;
+        const int j_first = r0 * KEYS + wave * 16 * TK;
+        const int j_end = min(r1 * KEYS, lim_hi);
+        const int steps = j_first < j_end ? (j_end - j_first + KEYS - 1) / KEYS : 0;
+        const int32_t* row = table + (int64_t)b * c.table_stride;
+        // the block's positions in whole 16s, those past the last one seen moved back onto it
+        auto base16 = [&](int j) { return min(j, (lim_hi - 1) & ~15); };
+        struct Ids {
+            int p[TK];
+        };
+        auto ids_of = [&](int s) __attribute__((always_inline)) {
+            Ids d;
+#pragma unroll
+            for (int t = 0; t < TK; t++)
+                d.p[t] = __builtin_amdgcn_readfirstlane(row[base16(j_first + s * KEYS + 16 * t) >> c.shift]);
+            return d;
+        };
+        struct Buf {
+            piece k[TK][KS];
+            vec v[4 * TK][VN];
+        };
+        const uint32_t kof = (uint32_t)(col * D + L::PIECE * g) * EB;  // + 64 s bytes
+        const uint32_t vof = (uint32_t)(4 * g * D + VE * col) * EB;    // + e D EB + 16 VE i EB
+        uint32_t vofs[VN];
+#pragma unroll
+        for (int i = 0; i < VN; i++) vofs[i] = 16 * VE * i + VE * col < D ? vof + 16 * VE * i * EB : (uint32_t)(4 * g * D) * EB;
+        auto load = [&](int s, const Ids& d, Buf& f) __attribute__((always_inline)) {
+#pragma unroll
+            for (int t = 0; t < TK; t++) {
+                const int j = base16(j_first + s * KEYS + 16 * t);
+                const int p = (uint32_t)d.p[t] < (uint32_t)c.n_pages ? d.p[t] : 0;
+                const int64_t at = (p * c.page_elems + (int64_t)(j & (page - 1)) * D) * EB + head;
+                const char *kb = kp + at, *vb = vp + at;
+#pragma unroll
+                for (int i = 0; i < KS; i++) {
+                    if (FULL || 4 * L::PIECE * (i + 1) <= D) {
+                        f.k[t][i] = *reinterpret_cast<const piece*>(kb + kof + 64 * i);
+                    } else {
+                        f.k[t][i] = piece{};
+                        if (4 * L::PIECE * i + L::PIECE * g < D) f.k[t][i] = *reinterpret_cast<const piece*>(kb + kof + 64 * i);
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+#pragma unroll
+                    for (int i = 0; i < VN; i++)
+                        f.v[4 * t + e][i] = *reinterpret_cast<const vec*>(vb + (FULL ? vof + 16 * VE * i * EB : vofs[i]) + e * D * EB);
+            }
+        };
+        float m = -INFINITY, l = 0.f;
+        floatx4 acc[NA];
+#pragma unroll
+        for (int i = 0; i < NA; i++) acc[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+
+        auto compute = [&](int s, const Ids& d, Buf& f) __attribute__((always_inline)) {
+            const int j0 = j_first + s * KEYS;
+            floatx4 st[TK];
+#pragma unroll
+            for (int t = 0; t < TK; t++) {
+                floatx4 z[2] = {floatx4{0.f, 0.f, 0.f, 0.f}, floatx4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+                for (int i = 0; i < KS; i++) {
+                    if constexpr (H16) {
+#pragma unroll
+                        for (int p = 0; p < QP; p++) z[p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.k[t][i], qf[p][i], z[p], 0, 0, 0);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) z[e & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(f.k[t][i][e], qf[0][i][e], z[e & 1], 0, 0, 0);
+                    }
+                }
+                st[t] = QP == 2 || !H16 ? z[0] + z[1] : z[0];
+            }
+            bool odd = false;  // pages that do not exist
+#pragma unroll
+            for (int t = 0; t < TK; t++) odd |= (uint32_t)d.p[t] >= (uint32_t)c.n_pages;
+            const bool edge = j0 + 16 * TK > lim_lo;
+            bool fix = false;
+            if (edge || odd) {
+#pragma unroll
+                for (int t = 0; t < TK; t++) {
+                    const bool none = (uint32_t)d.p[t] >= (uint32_t)c.n_pages;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int j = j0 + 16 * t + 4 * g + e;
+                        if (none) st[t][e] = NAN;
+                        if (j >= lim) st[t][e] = -INFINITY;
+                        // values that no row sees (or of no page) are zeros: a weight of 0 would
+                        // not silence an infinity
+                        if (none || j >= lim_hi) {
+#pragma unroll
+                            for (int i = 0; i < VN; i++) f.v[4 * t + e][i] = vec{};
+                        }
+                    }
+                }
+                // those that only some rows see: infinities and NaN are taken out of the product
+                // and added to the rows that see them
+                if (lim_lo < lim_hi) {
+                    uint32_t wild = 0;
+#pragma unroll
+                    for (int e = 0; e < 4 * TK; e++)
+#pragma unroll
+                        for (int i = 0; i < VN; i++) {
+                            words u = __builtin_bit_cast(words, f.v[e][i]);
+#pragma unroll
+                            for (int y = 0; y < (int)(sizeof(vec) / 4); y++) {
+                                const uint32_t z = not_finite<KVT>(u[y]);
+                                wild |= z;
+                                u[y] &= ~z;
+                            }
+                            f.v[e][i] = __builtin_bit_cast(vec, u);
+                        }
+                    fix = __ballot(wild != 0) != 0;
+                }
+            }
+            float mt = st[0][0];
+#pragma unroll
+            for (int t = 0; t < TK; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) mt = fmaxf(mt, st[t][e]);
+            mt = lane_pair_max<16>(mt);
+            mt = lane_pair_max<32>(mt);
+            const float mn = fmaxf(m, mt), ms = mn == -INFINITY ? 0.f : mn;
+            if (__ballot(mn != m)) {
+                const float al = __builtin_amdgcn_exp2f((m - ms) * cs);
+                l *= al;
+#pragma unroll
+                for (int i = 0; i < NA; i++) acc[i] *= al;
+            }
+            m = mn;
+#pragma unroll
+            for (int t = 0; t < TK; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    st[t][e] = __builtin_amdgcn_exp2f(H16 ? fmaf(st[t][e] - ms, cs, 15.0f) : (st[t][e] - ms) * cs);
+                    l += st[t][e];
+                }
+            if constexpr (H16) {
+                constexpr int KM = TK == 1 ? 1 : TK / 2;  // matrix instructions per operand
+                typedef std::conditional_t<TK == 1, half4v, half8> op;
+                constexpr int N = TK == 1 ? 4 : 8;
+#pragma unroll
+                for (int u = 0; u < KM; u++) {
+                    op hi, lo;
+#pragma unroll
+                    for (int e = 0; e < N; e++) {
+                        const float p = st[2 * u + e / 4][e % 4];
+                        hi[e] = (_Float16)p;
+                        lo[e] = (_Float16)(p - (float)hi[e]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < VN; i++)
+#pragma unroll
+                        for (int y = 0; y < VE; y++) {
+                            op av;
+#pragma unroll
+                            for (int e = 0; e < N; e++) av[e] = f.v[N * u + e][i][y];
+                            floatx4& o = acc[i * VE + y];
+                            if constexpr (TK == 1) {
+                                o = __builtin_amdgcn_mfma_f32_16x16x16f16(av, hi, o, 0, 0, 0);
+                                o = __builtin_amdgcn_mfma_f32_16x16x16f16(av, lo, o, 0, 0, 0);
+                            } else {
+                                o = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, hi, o, 0, 0, 0);
+                                o = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, lo, o, 0, 0, 0);
+                            }
+                        }
+                }
+            } else {
+#pragma unroll
+                for (int t = 0; t < TK; t++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+#pragma unroll
+                        for (int i = 0; i < VN; i++)
+#pragma unroll
+                            for (int y = 0; y < VE; y++)
+                                acc[i * VE + y] = __builtin_amdgcn_mfma_f32_16x16x4f32(f.v[4 * t + e][i][y], st[t][e], acc[i * VE + y], 0, 0, 0);
+            }
+            if (fix) {
+#pragma unroll 1
+                for (int k = 0; k < 16 * TK; k++) {
+                    int dims = D;
+                    asm volatile("" : "+s"(dims));  // its comparisons stay here
+                    const int j = j0 + k;
+                    if (j >= lim_hi) break;
+                    const int p = row[j >> c.shift];
+                    if ((uint32_t)p >= (uint32_t)c.n_pages || j >= lim) continue;
+                    const KVT* vr = reinterpret_cast<const KVT*>(vp + (p * c.page_elems + (int64_t)(j & (page - 1)) * D) * EB + head);
+#pragma unroll
+                    for (int i = 0; i < NA; i++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const int dim = 16 * VE * (i / VE) + VE * (4 * g + e) + i % VE;
+                            const float v = FULL || dim < dims ? (float)vr[dim] : 0.f;
+                            acc[i][e] += __uint_as_float(__float_as_uint(v) & not_finite<float>(__float_as_uint(v)));
+                        }
+                }
+            }
+        };
+
+        if (steps > 0) {
+            Buf f0, f1;
+            Ids d0 = ids_of(0), d1 = d0;
+            load(0, d0, f0);
+            if (steps > 1) d1 = ids_of(1);
+            for (int s = 0; s < steps; s += 2) {
+                if (s + 1 < steps) load(s + 1, d1, f1);
+                __builtin_amdgcn_sched_barrier(0);
+                Ids d2 = d0;
+                if (s + 2 < steps) d2 = ids_of(s + 2);
+                compute(s, d0, f0);
+                __builtin_amdgcn_sched_barrier(0);
+                if (s + 1 >= steps) break;
+                if (s + 2 < steps) load(s + 2, d2, f0);
+                __builtin_amdgcn_sched_barrier(0);
+                d0 = d2;
+                Ids d3 = d1;
+                if (s + 3 < steps) d3 = ids_of(s + 3);
+                compute(s + 1, d1, f1);
+                __builtin_amdgcn_sched_barrier(0);
+                d1 = d3;
+            }
+        }
+        l = lane_pair_sum<16>(l);
+        l = lane_pair_sum<32>(l);
+        __syncthreads();  // so is free
+        if (g == 0) so[wave][col][DP] = m, so[wave][col][DP + 1] = l, so[wave][col][DP + 2] = cs;
+        // lane: dimensions 16 VE i + VE (4 g + e) + y of row col
+#pragma unroll
+        for (int i = 0; i < VN; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+#pragma unroll
+                for (int y = 0; y < VE; y += 4)
+                    *reinterpret_cast<floatx4*>(&so[wave][col][16 * VE * i + VE * (4 * g + e) + y]) =
+                        floatx4{acc[i * VE + y][e], acc[i * VE + y + 1][e], acc[i * VE + y + 2][e], acc[i * VE + y + 3][e]};
+        __syncthreads();
+        // thread: row tr, every 16th float4 of it
+        const int tr = threadIdx.x >> 4, tc = threadIdx.x & 15;
+        const float rc = so[0][tr][DP + 2];
+        float M = -INFINITY;
+#pragma unroll
+        for (int v = 0; v < 4; v++) M = fmaxf(M, so[v][tr][DP]);
+        const float Ms = M == -INFINITY ? 0.f : M;
+        float fw[4], sum = 0.f;
+#pragma unroll
+        for (int v = 0; v < 4; v++) fw[v] = __builtin_amdgcn_exp2f((so[v][tr][DP] - Ms) * rc), sum = fmaf(so[v][tr][DP + 1], fw[v], sum);
+        const bool whole = r0 == 0 && r1 == w.rounds;
+        const int orow = tile * 16 + tr, oq = orow / G;
+        float* rec = a.ws + (int64_t)(2 * run + (r0 == 0 ? 1 : 0)) * 16 * (D + 4) + tr * (D + 4);
+        const int64_t sees = shown + oq;
+        const float inv = sees > len ? NAN : 1.0f / sum;
+        QT* op = static_cast<QT*>(a.out) + ((int64_t)(first + oq) * a.hq + h * G + orow - oq * G) * D;
+        if (orow < rows) {
+#pragma unroll
+            for (int i = 0; i < (DP + 63) / 64; i++) {
+                const int dim = 64 * i + 4 * tc;
+                if (dim >= D) continue;
+                floatx4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int v = 0; v < 4; v++) {
+                    const floatx4 z = *reinterpret_cast<const floatx4*>(&so[v][tr][dim]);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) o[e] = fmaf(z[e], fw[v], o[e]);
+                }
+                if (!whole) {
+                    *reinterpret_cast<floatx4*>(rec + dim) = o;
+                } else {
+                    if (sees <= 0) o = floatx4{0.f, 0.f, 0.f, 0.f};
+                    else o *= inv;
+                    if constexpr (std::is_same_v<QT, float>) *reinterpret_cast<floatx4*>(op + dim) = o;
+                    else *reinterpret_cast<half4v*>(op + dim) = half4v{(_Float16)o[0], (_Float16)o[1], (_Float16)o[2], (_Float16)o[3]};
+                }
+            }
+            if (!whole && tc == 0) *reinterpret_cast<floatx4*>(rec + D) = floatx4{M, sum, rc, 0.f};
+        }
+    }
+}
+
+// Tiles that several runs share, and those without a position: one workgroup per (sequence, KV
+// head, tile) that there can be, in the line's order.
+template <typename QT>
+__global__ __launch_bounds__(256) void k_paged_join(const PagedAttn a, int keys, int runs) {
+    const PagedCache& c = a.c;
+    const int lane = threadIdx.x & 63, G = a.G, D = c.D;
+    int64_t total = 0, units = 0, at = -1, nth = 0;
+    int b = -1;
+    for (int base = 0; base < c.batch; base += 64) {
+        Work w{0, 0};
+        if (base + lane < c.batch) w = work_of(c, base + lane, G, keys);
+        const int64_t wu = (int64_t)c.hkv * w.tiles, ww = wu * w.rounds, iu = lane_prefix(wu), iw = lane_prefix(ww);
+        const uint64_t hit = __ballot(blockIdx.x < units + iu);
+        if (b < 0 && hit) {
+            const int i = __builtin_ctzll(hit);
+            b = base + i;
+            nth = blockIdx.x - (units + lane_value(iu, i) - lane_value(wu, i));
+            at = total + lane_value(iw, i) - lane_value(ww, i);
+        }
+        units += lane_value(iu, 63);
+        total += lane_value(iw, 63);
+    }
+    if (b < 0) return;
+    const Work w = work_of(c, b, G, keys);
+    const int64_t len_run = total <= runs ? 1 : (total + runs - 1) / runs;
+    const int64_t x = at + nth * w.rounds;
+    const int64_t run0 = x / len_run, run1 = w.rounds ? (x + w.rounds - 1) / len_run : run0;
+    if (w.rounds && run0 == run1) return;
+    const int h = (int)(nth / w.tiles), tile = (int)(nth - (int64_t)h * w.tiles);
+    int first;
+    bool past;
+    const int n = paged_rows(c, b, &first), len = paged_len(c, b, &past), rows = n * G;
+    const int tr = threadIdx.x >> 4, tc = threadIdx.x & 15, orow = tile * 16 + tr, oq = orow / G;
+    if (orow >= rows) return;
+    const int64_t sees = (int64_t)max(c.lens[b], 0) - n + 1 + oq;
+    const float* rec = a.ws + (2 * run0 + 1) * 16 * (D + 4) + tr * (D + 4);  // the next ones: slot 0 of run0 + 1, ...
+    const int64_t step = (int64_t)2 * 16 * (D + 4);
+    const int parts = w.rounds ? (int)(run1 - run0 + 1) : 0;
+    auto part = [&](int i) { return i == 0 ? rec : rec + i * step - 16 * (D + 4); };
+    float M = -INFINITY;
+    for (int i = 0; i < parts; i++) M = fmaxf(M, part(i)[D]);
+    const float Ms = M == -INFINITY ? 0.f : M;
+    floatx4 o[4] = {};
+    float sum = 0.f;
+    for (int i = 0; i < parts; i++) {
+        const float* p = part(i);
+        const floatx4 mlc = *reinterpret_cast<const floatx4*>(p + D);
+        const float f = __builtin_amdgcn_exp2f((mlc[0] - Ms) * mlc[2]);
+        sum = fmaf(mlc[1], f, sum);
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+            if (64 * u + 4 * tc < D) {
+                const floatx4 z = *reinterpret_cast<const floatx4*>(p + 64 * u + 4 * tc);
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[u][e] = fmaf(z[e], f, o[u][e]);
+            }
+    }
+    const float inv = sees > len ? NAN : 1.0f / sum;
+    QT* op = static_cast<QT*>(a.out) + ((int64_t)(first + oq) * a.hq + h * G + orow - oq * G) * D;
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+        const int dim = 64 * u + 4 * tc;
+        if (dim >= D) break;
+        const floatx4 v = sees <= 0 ? floatx4{0.f, 0.f, 0.f, 0.f} : o[u] * inv;
+        if constexpr (std::is_same_v<QT, float>) *reinterpret_cast<floatx4*>(op + dim) = v;
+        else *reinterpret_cast<half4v*>(op + dim) = half4v{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
+    }
+}
+
+size_t paged_attention_workspace(int64_t batch, int64_t rows, int hq, int hkv, int D) {
+    return (size_t)RUNS * 2 * 16 * (D + 4) * sizeof(float);
+}
+
+template <typename KVT, typename QT, int DP, int TK, bool FULL>
+static int launch_tile_of(const PagedAttn& a, hipStream_t s) {
+    constexpr int KEYS = Tile<KVT, QT, DP, TK>::KEYS;
+    // as many runs as there can be rounds, up to two workgroups per CU
+    const int64_t units = a.c.hkv * (a.c.cu ? cdiv((int64_t)a.c.rows * a.G, 16) + a.c.batch : (int64_t)a.c.batch * cdiv(a.G, 16));
+    const int64_t most = units * cdiv(a.c.capacity, KEYS);
+    const int runs = (int)(most < RUNS ? most : RUNS);
+    k_paged_tile<KVT, QT, DP, TK, FULL><<<dim3((unsigned)runs), 256, 0, s>>>(a, a.c.table, static_cast<const char*>(a.c.k), static_cast<const char*>(a.c.v));
+    k_paged_join<QT><<<dim3((unsigned)units), 256, 0, s>>>(a, KEYS, runs);
     hipError_t e = hipGetLastError();
     return e == hipSuccess ? TL_HIP_OK : hip_fail(e, "paged attention launch");
+}
+
+template <typename KVT, typename QT, int DP, int TK>
+static int launch_tile(const PagedAttn& a, hipStream_t s) {
+    return a.c.D == DP ? launch_tile_of<KVT, QT, DP, TK, true>(a, s) : launch_tile_of<KVT, QT, DP, TK, false>(a, s);
+}
+
+template <typename KVT, typename QT>
+static int launch_kind(const PagedAttn& a, hipStream_t s) {
+    constexpr bool H16 = std::is_same_v<KVT, _Float16>;
+    if (a.c.D <= 64) return launch_tile<KVT, QT, 64, 2>(a, s);
+    if (a.c.D == 128) return launch_tile_of<KVT, QT, 128, H16 ? 2 : 1, true>(a, s);
+    if (a.c.D < 128) return launch_tile_of<KVT, QT, 128, 1, false>(a, s);  // (two at a time: registers spill)
+    return launch_tile<KVT, QT, 256, 1>(a, s);
+}
+
+int launch_paged_attention(const PagedAttn& a, bool q16, bool kv16, hipStream_t s) {
+    if (q16) return launch_kind<_Float16, _Float16>(a, s);
+    if (kv16) return launch_kind<_Float16, float>(a, s);
+    return launch_kind<float, float>(a, s);
 }
 
 }  // namespace tlhip
