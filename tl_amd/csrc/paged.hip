@@ -161,7 +161,7 @@ static int check_attention(PagedAttn* a, const void* q, int q_dtype, int64_t q_s
         set_error(TL_HIP_ERR_NULL, "NullPointerError: q, pages, page_table, kv_lens or out");
         return TL_HIP_ERR_NULL;
     }
-    if (rows * (hq / hkv) > (1 << 30)) return arg_error("n_tokens * n_heads / n_kv_heads must be at most 2^30");
+    if (rows * hq > (1 << 26) || batch * hkv > (1 << 22)) return arg_error("n_tokens * n_heads must be at most 2^26, batch * n_kv_heads 2^22");
     const int per16 = q_dtype == TL_HIP_F16 ? 8 : 4;
     if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out)) return arg_error("q, pages and out must be 16-byte aligned");
     if (q_stride % per16 || q_stride < (int64_t)hq * D || q_stride > (int64_t(1) << 40))

@@ -5,6 +5,7 @@
 //   l = sum_j 2^(c (s_j - m)),  o = sum_j 2^(c (s_j - m)) v_j,
 // both multiplied by 2^(c (m_old - m_new)) where the maximum rises; out = o / l.  Parts of the
 // positions join the same way.
+#include "gemm_common.h"
 #include "paged.h"
 
 #include <cfloat>
@@ -490,6 +491,298 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_tile(
     }
 }
 
+// ---- prompts over f16 caches -------------------------------------------------------------
+// A workgroup takes 128 rows, a wavefront 32 of them; 64 positions (32 at head sizes past 128) at
+// a time reach LDS by DMA, the next ones under the work on these.  S^T = K Q^T and
+// O^T += V^T P^T on v_mfma_f32_32x32x16_f16: lane (col, hf) = (l % 32, l / 32) holds row col's scores at
+// keys 8 (i / 4) + 4 hf + i % 4 of 32, which are the k slots of the second product as they stand;
+// V^T is read from row-major V by the transposing LDS reads.  Rows that nothing asks for, of
+// positions past the last one seen and of dimensions past head_dim, lie outside the buffer
+// resources and arrive as zeros.
+// 16-byte chunks of K rows are spread by the row, so that 16 rows of one chunk lie in 16
+// different places of the banks; chunks of V rows by quarters, for four rows of 64 bytes.
+template <int DP>
+struct PromptTile {
+    static constexpr int KT = DP > 128 ? 32 : 64;
+    static constexpr int CPR = DP / 8;       // chunks per row
+    static constexpr int U = KT * CPR / 256; // DMA instructions per wavefront and operand
+    __device__ static int spread_k(int r) { return CPR == 8 ? (r >> 1) & 7 : r & 15; }
+    __device__ static int spread_v(int r) { return CPR == 8 ? ((r >> 1) & 1) << 2 : (r & 3) << 2; }
+};
+
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef short short4v __attribute__((ext_vector_type(4)));
+
+template <typename QT, int DP>
+__global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_prompt(
+    const PagedAttn a, const int32_t* __restrict__ table, const char* __restrict__ kp, const char* __restrict__ vp) {
+    using L = PromptTile<DP>;
+    constexpr int KT = L::KT, CPR = L::CPR, U = L::U, RPW = KT / 4;
+    constexpr int QP = std::is_same_v<QT, float> ? 2 : 1;  // f16 parts of a query, and of a weight
+    constexpr int KS = DP / 16, DT = DP / 32, ST = KT / 32;
+    struct Stage {
+        uint4 k[KT * CPR], v[KT * CPR];
+    };
+    __shared__ __attribute__((aligned(16))) Stage S0, S1;
+    const PagedCache& c = a.c;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, hf = lane >> 5;
+    const int G = a.G, D = c.D, page = 1 << c.shift;
+
+    // tiles from the last one back: of one sequence the longest first
+    const int h = blockIdx.x % c.hkv, back = blockIdx.x / c.hkv;
+    auto tiles_of = [&](int b) {
+        int f;
+        return b < c.batch ? (paged_rows(c, b, &f) * G + 127) >> 7 : 0;
+    };
+    int64_t total = 0, incl = 0, mine = 0;
+    for (int base = 0; base < c.batch; base += 64) {
+        mine = tiles_of(base + lane);
+        incl = lane_prefix(mine);
+        total += lane_value(incl, 63);
+    }
+    const int64_t nth = total - 1 - back;
+    if (nth < 0) return;
+    int b = 0, tile = 0;
+    int64_t before = 0;
+    for (int base = 0;; base += 64) {
+        if (c.batch > 64) {
+            mine = tiles_of(base + lane);
+            incl = lane_prefix(mine);
+        }
+        const uint64_t hit = __ballot(nth < before + incl);
+        if (hit) {
+            const int at = __builtin_ctzll(hit);
+            b = base + at;
+            tile = (int)(nth - (before + lane_value(incl, at) - lane_value(mine, at)));
+            break;
+        }
+        before += lane_value(incl, 63);
+    }
+    b = __builtin_amdgcn_readfirstlane(b);
+    tile = __builtin_amdgcn_readfirstlane(tile);
+
+    int first;
+    bool past;
+    const int n = paged_rows(c, b, &first), len = paged_len(c, b, &past), rows = n * G;
+    const int64_t shown = (int64_t)max(c.lens[b], 0) - n + 1;  // positions that query 0 sees
+    auto limit = [&](int row) { return (int)max(min(shown + min(row, rows - 1) / G, (int64_t)len), (int64_t)0); };
+    const int w0 = tile * 128 + wave * 32, r = min(w0 + col, rows - 1), qi = r / G, qh = h * G + r - qi * G;
+    const int lim = limit(r), lim_lo = limit(w0), lim_hi = limit(w0 + 31), last = limit(tile * 128 + 127);
+    const bool live = w0 < rows;
+
+    // this lane's part of its row: dimensions 16 s + 8 hf ..
+    const QT* qp = static_cast<const QT*>(a.q) + (int64_t)(first + qi) * a.q_stride + qh * D;
+    const float sign = a.scale < 0.f ? -1.f : a.scale > 0.f ? 1.f : 0.f;
+    float cs = fminf(fabsf(a.scale) * 1.44269504088896341f, FLT_MAX);
+    half8 qf[QP][KS];
+    if constexpr (QP == 2) {
+        float top = 0.f;
+        floatx4 qv[KS][2];
+#pragma unroll
+        for (int s = 0; s < KS; s++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                qv[s][e] = 16 * s + 8 * hf < D ? reinterpret_cast<const floatx4*>(qp + 16 * s + 8 * hf)[e] : floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < 4; i++) top = fmaxf(top, fabsf(qv[s][e][i]));
+            }
+        top = lane_pair_max<32>(top);
+        const int up = top > 0.f && top <= FLT_MAX ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
+        cs = fminf(ldexpf(fabsf(a.scale) * 1.44269504088896341f, -up), FLT_MAX);
+#pragma unroll
+        for (int s = 0; s < KS; s++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float f = ldexpf(qv[s][i / 4][i % 4] * sign, up);
+                qf[0][s][i] = (_Float16)f;
+                qf[1][s][i] = (_Float16)(f - (float)qf[0][s][i]);
+            }
+    } else {
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            half8 z = {};
+            if (16 * s + 8 * hf < D) z = *reinterpret_cast<const half8*>(qp + 16 * s + 8 * hf);
+#pragma unroll
+            for (int i = 0; i < 8; i++) qf[0][s][i] = z[i] * (_Float16)sign;
+        }
+    }
+    cs = fmaxf(cs, FLT_MIN);
+
+    // DMA: this wavefront's rows RPW wave .. of a tile, all in one page
+    uint32_t ko[U], vo[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int at = u * 64 + lane, rr = at / CPR, ch = at % CPR, tr = wave * RPW + rr;
+        const int ck = ch ^ L::spread_k(tr), cv = ch ^ L::spread_v(tr);
+        ko[u] = 8 * ck < D ? (uint32_t)(rr * D + 8 * ck) * 2 : 0x7FFFFFF0u;
+        vo[u] = 8 * cv < D ? (uint32_t)(rr * D + 8 * cv) * 2 : 0x7FFFFFF0u;
+    }
+    const int32_t* row = table + (int64_t)b * c.table_stride;
+    const int64_t head = (int64_t)h * page * D;
+    auto page_of = [&](int j0) { return __builtin_amdgcn_readfirstlane(row[min(j0 + wave * RPW, last - 1) >> c.shift]); };
+    auto issue = [&](int j0, int pid, Stage& st) __attribute__((always_inline)) {
+        const int j = j0 + wave * RPW;
+        const bool none = (uint32_t)pid >= (uint32_t)c.n_pages;
+        const int64_t at = ((none ? 0 : pid) * c.page_elems + head + (int64_t)(j & (page - 1)) * D) * 2;
+        const uint32_t bytes = none ? 0u : (uint32_t)max(min(last - j, RPW), 0) * D * 2;
+        const __amdgpu_buffer_rsrc_t rk = buf_rsrc(kp + at, bytes), rv = buf_rsrc(vp + at, bytes);
+        if (!none) {
+#pragma unroll
+            for (int u = 0; u < U; u++) buf_dma16(rk, ko[u], 0, &st.k[(wave * U + u) * 64]);
+        } else {  // a page that does not exist: NaN scores over zero values
+#pragma unroll
+            for (int u = 0; u < U; u++) st.k[(wave * U + u) * 64 + lane] = make_uint4(0x7E007E00u, 0x7E007E00u, 0x7E007E00u, 0x7E007E00u);
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) buf_dma16(rv, vo[u], 0, &st.v[(wave * U + u) * 64]);
+    };
+
+    float m = -INFINITY, l = 0.f;
+    floatx16 acc[DT];
+#pragma unroll
+    for (int i = 0; i < DT; i++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) acc[i][e] = 0.f;
+
+    const int trow = 4 * hf + ((lane & 15) >> 2);  // the key of this lane's address in a transposing read
+    auto compute = [&](int j0, const Stage& st, auto edge) __attribute__((always_inline)) {
+        constexpr bool EDGE = decltype(edge)::value;
+        floatx16 sc[ST];
+#pragma unroll
+        for (int t = 0; t < ST; t++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) sc[t][e] = 0.f;
+#pragma unroll
+        for (int s = 0; s < KS; s++)
+#pragma unroll
+            for (int t = 0; t < ST; t++) {
+                const int kr = 32 * t + col;
+                const half8 kf = __builtin_bit_cast(half8, st.k[kr * CPR + ((2 * s + hf) ^ L::spread_k(kr))]);
+#pragma unroll
+                for (int p = 0; p < QP; p++) sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[p][s], sc[t], 0, 0, 0);
+            }
+        if constexpr (EDGE) {
+#pragma unroll
+            for (int t = 0; t < ST; t++)
+#pragma unroll
+                for (int e = 0; e < 16; e++)
+                    if (j0 + 32 * t + 8 * (e / 4) + 4 * hf + e % 4 >= lim) sc[t][e] = -INFINITY;
+        }
+        float mt = sc[0][0];
+#pragma unroll
+        for (int t = 0; t < ST; t++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) mt = fmaxf(mt, sc[t][e]);
+        mt = lane_pair_max<32>(mt);
+        // the maximum is raised only where weights would pass 2^8 (times 2^7, f16's range)
+        if (__ballot((mt - m) * cs > 8.0f)) {
+            const float mn = fmaxf(m, mt), al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * cs);
+            m = mn;
+            l *= al;
+#pragma unroll
+            for (int i = 0; i < DT; i++) acc[i] *= al;
+        }
+        const float ms = m == -INFINITY ? 0.f : m, bias = fmaf(-ms, cs, 7.0f);
+        half8 pf[QP][KT / 16];
+#pragma unroll
+        for (int t = 0; t < ST; t++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const float p = __builtin_amdgcn_exp2f(QP == 2 ? fmaf(sc[t][e] - ms, cs, 7.0f) : fmaf(sc[t][e], cs, bias));
+                l += p;
+                const _Float16 hi = (_Float16)p;
+                pf[0][2 * t + e / 8][e % 8] = hi;
+                if constexpr (QP == 2) pf[1][2 * t + e / 8][e % 8] = (_Float16)(p - (float)hi);
+            }
+        uint32_t wild = 0;
+        const _Float16* vh = reinterpret_cast<const _Float16*>(st.v);
+#pragma unroll
+        for (int s = 0; s < KT / 16; s++)
+#pragma unroll
+            for (int i = 0; i < DT; i++) {
+                const int ch = 4 * i + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
+                uint2 w[2];
+#pragma unroll
+                for (int y = 0; y < 2; y++) {
+                    const int kr = 16 * s + 8 * y + trow;
+                    const _Float16* p = vh + kr * DP + 8 * (ch ^ L::spread_v(kr)) + 4 * (lane & 1);
+                    w[y] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)p));
+                }
+                uint4 f = make_uint4(w[0].x, w[0].y, w[1].x, w[1].y);
+                if constexpr (EDGE) {  // infinities and NaN: added below to the rows that see them
+                    uint32_t* u = &f.x;
+#pragma unroll
+                    for (int y = 0; y < 4; y++) {
+                        const uint32_t z = not_finite<_Float16>(u[y]);
+                        wild |= z;
+                        u[y] &= ~z;
+                    }
+                }
+                const half8 vf = __builtin_bit_cast(half8, f);
+#pragma unroll
+                for (int p = 0; p < QP; p++) acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[p][s], acc[i], 0, 0, 0);
+            }
+        if constexpr (EDGE) {
+            if (__ballot(wild != 0)) {
+#pragma unroll 1
+                for (int k = 0; k < KT && j0 + k < last; k++) {
+                    if (j0 + k >= lim) continue;
+#pragma unroll
+                    for (int i = 0; i < DT; i++)
+#pragma unroll
+                        for (int e = 0; e < 16; e++) {
+                            const int d = 32 * i + 8 * (e / 4) + 4 * hf + e % 4;
+                            const uint32_t v = __float_as_uint((float)vh[k * DP + 8 * ((d >> 3) ^ L::spread_v(k)) + (d & 7)]);
+                            acc[i][e] += __uint_as_float(v & not_finite<float>(v));
+                        }
+                }
+            }
+        }
+    };
+
+    const int tiles = (last + KT - 1) / KT;
+    if (tiles > 0) {
+        int pid = page_of(0);
+        issue(0, pid, S0);
+        pid = page_of(KT);
+        auto step = [&](int t, const Stage& cur, Stage& next) __attribute__((always_inline)) {
+            __builtin_amdgcn_s_waitcnt(0xF70);  // vmcnt(0): this tile's DMA has landed
+            __syncthreads();
+            __builtin_amdgcn_sched_barrier(0);
+            if (t + 1 < tiles) {
+                issue((t + 1) * KT, pid, next);
+                pid = page_of((t + 2) * KT);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if (live && t * KT < lim_hi) {
+                if ((t + 1) * KT <= lim_lo) compute(t * KT, cur, std::false_type{});
+                else compute(t * KT, cur, std::true_type{});
+            }
+        };
+        for (int t = 0; t < tiles; t += 2) {
+            step(t, S0, S1);
+            if (t + 1 < tiles) step(t + 1, S1, S0);
+        }
+    }
+    l = lane_pair_sum<32>(l);
+    if (w0 + col >= rows) return;
+    const int64_t sees = shown + qi;
+    const float inv = sees > len ? NAN : 1.0f / l;
+    QT* op = static_cast<QT*>(a.out) + ((int64_t)(first + qi) * a.hq + qh) * D;
+#pragma unroll
+    for (int i = 0; i < DT; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int d = 32 * i + 8 * e + 4 * hf;
+            if (d >= D) continue;
+            floatx4 o = {acc[i][4 * e], acc[i][4 * e + 1], acc[i][4 * e + 2], acc[i][4 * e + 3]};
+            if (sees <= 0) o = floatx4{0.f, 0.f, 0.f, 0.f};
+            else o *= inv;
+            if constexpr (std::is_same_v<QT, float>) *reinterpret_cast<floatx4*>(op + d) = o;
+            else *reinterpret_cast<half4v*>(op + d) = half4v{(_Float16)o[0], (_Float16)o[1], (_Float16)o[2], (_Float16)o[3]};
+        }
+}
+
 // Tiles that several runs share, and those without a position: one workgroup per (sequence, KV
 // head, tile) that there can be, in the line's order.
 template <typename QT>
@@ -581,9 +874,24 @@ static int launch_tile(const PagedAttn& a, hipStream_t s) {
     return a.c.D == DP ? launch_tile_of<KVT, QT, DP, TK, true>(a, s) : launch_tile_of<KVT, QT, DP, TK, false>(a, s);
 }
 
+template <typename QT, int DP>
+static int launch_prompt(const PagedAttn& a, hipStream_t s) {
+    const int64_t units = a.c.hkv * (cdiv((int64_t)a.c.rows * a.G, 128) + a.c.batch);
+    k_paged_prompt<QT, DP><<<dim3((unsigned)units), 256, 0, s>>>(a, a.c.table, static_cast<const char*>(a.c.k), static_cast<const char*>(a.c.v));
+    hipError_t e = hipGetLastError();
+    return e == hipSuccess ? TL_HIP_OK : hip_fail(e, "paged attention launch");
+}
+
 template <typename KVT, typename QT>
 static int launch_kind(const PagedAttn& a, hipStream_t s) {
     constexpr bool H16 = std::is_same_v<KVT, _Float16>;
+    if constexpr (H16) {
+        if (a.c.cu && (int64_t)a.c.rows * a.G >= 128 * (int64_t)a.c.batch) {
+            if (a.c.D <= 64) return launch_prompt<QT, 64>(a, s);
+            if (a.c.D <= 128) return launch_prompt<QT, 128>(a, s);
+            return launch_prompt<QT, 256>(a, s);
+        }
+    }
     if (a.c.D <= 64) return launch_tile<KVT, QT, 64, 2>(a, s);
     if (a.c.D == 128) return launch_tile_of<KVT, QT, 128, H16 ? 2 : 1, true>(a, s);
     if (a.c.D < 128) return launch_tile_of<KVT, QT, 128, 1, false>(a, s);  // (two at a time: registers spill)
