@@ -158,8 +158,9 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_tile(
         const int64_t shown = (int64_t)max(c.lens[b], 0) - n + 1;  // positions that query 0 sees
         const int r = min(tile * 16 + col, rows - 1), qi = r / G, qh = h * G + r - qi * G;
         const int lim = (int)max(min(shown + qi, (int64_t)len), (int64_t)0);
-        const int lim_lo = (int)max(min(shown + tile * 16 / G, (int64_t)len), (int64_t)0);
-        const int lim_hi = (int)max(min(shown + min(tile * 16 + 15, rows - 1) / G, (int64_t)len), (int64_t)0);
+        // positions that every row, that any row sees
+        const int lim_lo = __builtin_amdgcn_readfirstlane((int)max(min(shown + tile * 16 / G, (int64_t)len), (int64_t)0));
+        const int lim_hi = __builtin_amdgcn_readfirstlane((int)max(min(shown + min(tile * 16 + 15, rows - 1) / G, (int64_t)len), (int64_t)0));
 
         const QT* qp = static_cast<const QT*>(a.q) + (int64_t)(first + qi) * a.q_stride + qh * D;
         float cs = fminf(fabsf(a.scale) * 1.44269504088896341f, FLT_MAX);
@@ -523,7 +524,7 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_prompt(
     struct Stage {
         uint4 k[KT * CPR], v[KT * CPR];
     };
-    __shared__ __attribute__((aligned(16))) Stage S0, S1;
+    __shared__ __attribute__((aligned(16))) Stage S[2];
     const PagedCache& c = a.c;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, hf = lane >> 5;
     const int G = a.G, D = c.D, page = 1 << c.shift;
@@ -566,8 +567,10 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_prompt(
     const int n = paged_rows(c, b, &first), len = paged_len(c, b, &past), rows = n * G;
     const int64_t shown = (int64_t)max(c.lens[b], 0) - n + 1;  // positions that query 0 sees
     auto limit = [&](int row) { return (int)max(min(shown + min(row, rows - 1) / G, (int64_t)len), (int64_t)0); };
+    auto uniform = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
     const int w0 = tile * 128 + wave * 32, r = min(w0 + col, rows - 1), qi = r / G, qh = h * G + r - qi * G;
-    const int lim = limit(r), lim_lo = limit(w0), lim_hi = limit(w0 + 31), last = limit(tile * 128 + 127);
+    const int lim = limit(r), lim_hi = uniform(limit(w0 + 31));
+    const int last = uniform(limit(tile * 128 + 127)), all = uniform(limit(tile * 128));  // positions that any, that every row sees
     const bool live = w0 < rows;
 
     // this lane's part of its row: dimensions 16 s + 8 hf ..
@@ -624,7 +627,7 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_prompt(
         const int j = j0 + wave * RPW;
         const bool none = (uint32_t)pid >= (uint32_t)c.n_pages;
         const int64_t at = ((none ? 0 : pid) * c.page_elems + head + (int64_t)(j & (page - 1)) * D) * 2;
-        const uint32_t bytes = none ? 0u : (uint32_t)max(min(last - j, RPW), 0) * D * 2;
+        const uint32_t bytes = (uint32_t)uniform(none ? 0 : max(min(last - j, RPW), 0) * D * 2);
         const __amdgpu_buffer_rsrc_t rk = buf_rsrc(kp + at, bytes), rv = buf_rsrc(vp + at, bytes);
         if (!none) {
 #pragma unroll
@@ -645,7 +648,7 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_prompt(
         for (int e = 0; e < 16; e++) acc[i][e] = 0.f;
 
     const int trow = 4 * hf + ((lane & 15) >> 2);  // the key of this lane's address in a transposing read
-    auto compute = [&](int j0, const Stage& st, auto edge) __attribute__((always_inline)) {
+    auto compute = [&](int j0, const char* st, auto edge) __attribute__((always_inline)) {
         constexpr bool EDGE = decltype(edge)::value;
         floatx16 sc[ST];
 #pragma unroll
@@ -657,7 +660,7 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_prompt(
 #pragma unroll
             for (int t = 0; t < ST; t++) {
                 const int kr = 32 * t + col;
-                const half8 kf = __builtin_bit_cast(half8, st.k[kr * CPR + ((2 * s + hf) ^ L::spread_k(kr))]);
+                const half8 kf = __builtin_bit_cast(half8, reinterpret_cast<const uint4*>(st)[kr * CPR + ((2 * s + hf) ^ L::spread_k(kr))]);
 #pragma unroll
                 for (int p = 0; p < QP; p++) sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[p][s], sc[t], 0, 0, 0);
             }
@@ -695,7 +698,7 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_prompt(
                 if constexpr (QP == 2) pf[1][2 * t + e / 8][e % 8] = (_Float16)(p - (float)hi);
             }
         uint32_t wild = 0;
-        const _Float16* vh = reinterpret_cast<const _Float16*>(st.v);
+        const _Float16* vh = reinterpret_cast<const _Float16*>(st + sizeof(Stage::k));
 #pragma unroll
         for (int s = 0; s < KT / 16; s++)
 #pragma unroll
@@ -740,29 +743,27 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_prompt(
         }
     };
 
-    const int tiles = (last + KT - 1) / KT;
+    const int tiles = (last + KT - 1) / KT, whole = all / KT;
     if (tiles > 0) {
         int pid = page_of(0);
-        issue(0, pid, S0);
+        issue(0, pid, S[0]);
         pid = page_of(KT);
-        auto step = [&](int t, const Stage& cur, Stage& next) __attribute__((always_inline)) {
+        auto step = [&](int t, auto edge) __attribute__((always_inline)) {
             __builtin_amdgcn_s_waitcnt(0xF70);  // vmcnt(0): this tile's DMA has landed
             __syncthreads();
             __builtin_amdgcn_sched_barrier(0);
             if (t + 1 < tiles) {
-                issue((t + 1) * KT, pid, next);
+                issue((t + 1) * KT, pid, S[(t + 1) & 1]);
                 pid = page_of((t + 2) * KT);
             }
             __builtin_amdgcn_sched_barrier(0);
-            if (live && t * KT < lim_hi) {
-                if ((t + 1) * KT <= lim_lo) compute(t * KT, cur, std::false_type{});
-                else compute(t * KT, cur, std::true_type{});
-            }
+            if (live && t * KT < lim_hi) compute(t * KT, reinterpret_cast<const char*>(&S[t & 1]), edge);
         };
-        for (int t = 0; t < tiles; t += 2) {
-            step(t, S0, S1);
-            if (t + 1 < tiles) step(t + 1, S1, S0);
-        }
+        int t = 0;
+#pragma unroll 1
+        for (; t < whole; t++) step(t, std::false_type{});
+#pragma unroll 1
+        for (; t < tiles; t++) step(t, std::true_type{});
     }
     l = lane_pair_sum<32>(l);
     if (w0 + col >= rows) return;
