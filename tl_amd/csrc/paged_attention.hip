@@ -24,15 +24,44 @@ typedef _Float16 half4v __attribute__((ext_vector_type(4)));
 // adds them in order.
 constexpr int RUNS = 512;  // at most: two workgroups per CU
 
+// Sequences base + lane: packed rows first .. first + n - 1, positions len that the table holds,
+// and `shown` positions that its row 0 sees (0 or fewer: none).
+struct Seq {
+    int first, n, len, shown;
+};
+struct Group {
+    Seq q;
+    int base;
+    __device__ __forceinline__ void load(const PagedCache& c, const int32_t* cu, const int32_t* lens, int from) {
+        base = from;
+        const int b = from + (int)__lane_id();
+        q = Seq{0, 0, 0, 0};
+        if (b >= c.batch) return;
+        int lo = b, hi = b + 1;
+        if (cu) lo = min(max(cu[b], 0), c.rows), hi = min(max(cu[b + 1], 0), c.rows);
+        const int n = min(max(lens[b], 0), INT32_MAX - 32);
+        q.first = lo, q.n = max(hi - lo, 0), q.len = min(n, c.capacity), q.shown = n - q.n + 1;
+    }
+    __device__ __forceinline__ Seq at(int b) const {
+        const int i = b - base;
+        return Seq{__builtin_amdgcn_readlane(q.first, i), __builtin_amdgcn_readlane(q.n, i), __builtin_amdgcn_readlane(q.len, i),
+                   __builtin_amdgcn_readlane(q.shown, i)};
+    }
+    // the same, from another group where b lies there
+    __device__ __forceinline__ Seq at(const PagedCache& c, const int32_t* cu, const int32_t* lens, int b) {
+        if (b - base >= 64) load(c, cu, lens, b & ~63);
+        return at(b);
+    }
+};
+// Positions that row i of a sequence sees.
+__device__ __forceinline__ int limit_of(const Seq& q, int i) { return max(min(q.shown + i, q.len), 0); }
+
 struct Work {
     int tiles, rounds;
 };
-__device__ __forceinline__ Work work_of(const PagedCache& c, int b, int G, int keys) {
-    bool past;
-    int first;
-    const int n = paged_rows(c, b, &first);
-    if (n == 0) return {0, 0};
-    return {(n * G + 15) >> 4, (paged_len(c, b, &past) + keys - 1) / keys};
+__device__ __forceinline__ Work work_of(const Seq& q, int G, int keys) {
+    if (q.n == 0) return {0, 0};
+    return {(q.n * G + 15) >> 4, (q.len + keys - 1) / keys};
 }
 __device__ __forceinline__ int64_t lane_value(int64_t v, int lane) {
     return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)v, lane) |
@@ -89,7 +118,8 @@ struct Tile {
 // make rows of the product that are not stored, and read the row's first elements).
 template <typename KVT, typename QT, int DP, int TK, bool FULL>
 __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_tile(
-    const PagedAttn a, const int32_t* __restrict__ table, const char* __restrict__ kp, const char* __restrict__ vp) {
+    const PagedAttn a, const int32_t* __restrict__ table, const int32_t* __restrict__ cu, const int32_t* __restrict__ lens,
+    const char* __restrict__ kp, const char* __restrict__ vp) {
     using L = Tile<KVT, QT, DP, TK>;
     constexpr int QP = L::QP, KS = L::KS, VE = L::VE, VN = L::VN, NA = L::NA, KEYS = L::KEYS, EB = sizeof(KVT);
     constexpr bool H16 = L::H16;
@@ -105,10 +135,11 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_tile(
     const int runs = gridDim.x, id = blockIdx.x;
     const int run = (runs & 7) == 0 ? (id & 7) * (runs >> 3) + (id >> 3) : id;
 
+    Group grp;
     int64_t total = 0, incl = 0, mine = 0;
     for (int base = 0; base < c.batch; base += 64) {
-        Work w{0, 0};
-        if (base + lane < c.batch) w = work_of(c, base + lane, G, KEYS);
+        grp.load(c, cu, lens, base);
+        const Work w = work_of(grp.q, G, KEYS);
         mine = (int64_t)c.hkv * w.tiles * w.rounds;
         incl = lane_prefix(mine);
         total += lane_value(incl, 63);
@@ -121,8 +152,8 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_tile(
     int64_t before = 0;  // line position of sequence b's first round
     for (int base = 0;; base += 64) {
         if (c.batch > 64) {
-            Work w{0, 0};
-            if (base + lane < c.batch) w = work_of(c, base + lane, G, KEYS);
+            grp.load(c, cu, lens, base);
+            const Work w = work_of(grp.q, G, KEYS);
             mine = (int64_t)c.hkv * w.tiles * w.rounds;
             incl = lane_prefix(mine);
         }
@@ -135,10 +166,10 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_tile(
         }
         before += lane_value(incl, 63);
     }
-    b = __builtin_amdgcn_readfirstlane(b);
 
     while (x < x1) {
-        const Work w = work_of(c, b, G, KEYS);
+        const Seq sq = grp.at(c, cu, lens, b);
+        const Work w = work_of(sq, G, KEYS);
         const int64_t here = (int64_t)c.hkv * w.tiles * w.rounds;
         if (x >= before + here) {
             before += here;
@@ -151,76 +182,32 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_tile(
         const int h = unit / w.tiles, tile = unit - h * w.tiles;
         x += r1 - r0;
 
-        // this lane's row
-        int first;
-        bool past;
-        const int n = paged_rows(c, b, &first), len = paged_len(c, b, &past), rows = n * G;
-        const int64_t shown = (int64_t)max(c.lens[b], 0) - n + 1;  // positions that query 0 sees
+        // this lane's row; positions that it, that every row and that any row sees
+        const int rows = sq.n * G;
         const int r = min(tile * 16 + col, rows - 1), qi = r / G, qh = h * G + r - qi * G;
-        const int lim = (int)max(min(shown + qi, (int64_t)len), (int64_t)0);
-        // positions that every row, that any row sees
-        const int lim_lo = __builtin_amdgcn_readfirstlane((int)max(min(shown + tile * 16 / G, (int64_t)len), (int64_t)0));
-        const int lim_hi = __builtin_amdgcn_readfirstlane((int)max(min(shown + min(tile * 16 + 15, rows - 1) / G, (int64_t)len), (int64_t)0));
+        const int lim = limit_of(sq, qi);
+        const int lim_lo = __builtin_amdgcn_readfirstlane(limit_of(sq, tile * 16 / G));
+        const int lim_hi = __builtin_amdgcn_readfirstlane(limit_of(sq, min(tile * 16 + 15, rows - 1) / G));
 
-        const QT* qp = static_cast<const QT*>(a.q) + (int64_t)(first + qi) * a.q_stride + qh * D;
-        float cs = fminf(fabsf(a.scale) * 1.44269504088896341f, FLT_MAX);
-        const float sign = a.scale < 0.f ? -1.f : a.scale > 0.f ? 1.f : 0.f;
-        typedef std::conditional_t<H16, half8, floatx4> qvec;
-        qvec qf[QP][KS];
-        if constexpr (H16) {
-            float qv[KS][8];
-            float top = 0.f;
+        const QT* qp = static_cast<const QT*>(a.q) + (int64_t)(sq.first + qi) * a.q_stride + qh * D;
+        constexpr int QV = sizeof(QT) * L::PIECE / 16;  // 16-byte words per piece of the row
+        uint4 qw[KS][QV];
 #pragma unroll
-            for (int s = 0; s < KS; s++) {
-                const bool in = 32 * s + 8 * g < D;
-                if constexpr (QP == 2) {
+        for (int s = 0; s < KS; s++)
 #pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        const floatx4 f = in ? reinterpret_cast<const floatx4*>(qp + 32 * s + 8 * g)[e] : floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                        for (int i = 0; i < 4; i++) qv[s][4 * e + i] = f[i] * sign, top = fmaxf(top, fabsf(f[i]));
-                    }
-                } else {
-                    half8 z = {};
-                    if (in) z = *reinterpret_cast<const half8*>(qp + 32 * s + 8 * g);
-#pragma unroll
-                    for (int i = 0; i < 8; i++) qf[0][s][i] = z[i] * (_Float16)sign;
-                }
+            for (int e = 0; e < QV; e++) {
+                qw[s][e] = make_uint4(0u, 0u, 0u, 0u);
+                if (FULL || 4 * L::PIECE * s + L::PIECE * g < D) qw[s][e] = reinterpret_cast<const uint4*>(qp + 4 * L::PIECE * s + L::PIECE * g)[e];
             }
-            if constexpr (QP == 2) {
-                top = lane_pair_max<16>(top);
-                top = lane_pair_max<32>(top);
-                // the row's largest entry to 2^14 .. 2^15
-                const int up = top > 0.f && top <= FLT_MAX ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
-                cs = fminf(ldexpf(fabsf(a.scale) * 1.44269504088896341f, -up), FLT_MAX);
-#pragma unroll
-                for (int s = 0; s < KS; s++)
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const float f = ldexpf(qv[s][i], up);
-                        qf[0][s][i] = (_Float16)f;
-                        qf[1][s][i] = (_Float16)(f - (float)qf[0][s][i]);
-                    }
-            }
-        } else {
-#pragma unroll
-            for (int s = 0; s < KS; s++) {
-                floatx4 f = {};
-                if (16 * s + 4 * g < D) f = *reinterpret_cast<const floatx4*>(qp + 16 * s + 4 * g);
-#pragma unroll
-                for (int i = 0; i < 4; i++) qf[0][s][i] = f[i] * sign;
-            }
-        }
-        cs = fmaxf(cs, FLT_MIN);
 
-        // positions of this wavefront: blocks of 16 TK from j_of(0), every KEYS
+        // positions of this wavefront: blocks of 16 TK from j_first on, every KEYS
         const int64_t head = (int64_t)h * page * D * EB;
         const int j_first = r0 * KEYS + wave * 16 * TK;
         const int j_end = min(r1 * KEYS, lim_hi);
         const int steps = j_first < j_end ? (j_end - j_first + KEYS - 1) / KEYS : 0;
         const int32_t* row = table + (int64_t)b * c.table_stride;
         // the block's positions in whole 16s, those past the last one seen moved back onto it
-        auto base16 = [&](int j) { return min(j, (lim_hi - 1) & ~15); };
+        auto base16 = [&](int j) { return max(min(j, (lim_hi - 1) & ~15), 0); };
         struct Ids {
             int p[TK];
         };
@@ -250,19 +237,56 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_tile(
 #pragma unroll
                 for (int i = 0; i < KS; i++) {
                     if (FULL || 4 * L::PIECE * (i + 1) <= D) {
-                        f.k[t][i] = *reinterpret_cast<const piece*>(kb + kof + 64 * i);
+                        f.k[t][i] = __builtin_nontemporal_load(reinterpret_cast<const piece*>(kb + kof + 64 * i));
                     } else {
                         f.k[t][i] = piece{};
-                        if (4 * L::PIECE * i + L::PIECE * g < D) f.k[t][i] = *reinterpret_cast<const piece*>(kb + kof + 64 * i);
+                        if (4 * L::PIECE * i + L::PIECE * g < D) f.k[t][i] = __builtin_nontemporal_load(reinterpret_cast<const piece*>(kb + kof + 64 * i));
                     }
                 }
 #pragma unroll
                 for (int e = 0; e < 4; e++)
 #pragma unroll
                     for (int i = 0; i < VN; i++)
-                        f.v[4 * t + e][i] = *reinterpret_cast<const vec*>(vb + (FULL ? vof + 16 * VE * i * EB : vofs[i]) + e * D * EB);
+                        f.v[4 * t + e][i] = __builtin_nontemporal_load(reinterpret_cast<const vec*>(vb + (FULL ? vof + 16 * VE * i * EB : vofs[i]) + e * D * EB));
             }
         };
+        Buf f0, f1;
+        Ids d0 = ids_of(0), d1 = ids_of(max(min(1, steps - 1), 0));
+        __builtin_amdgcn_sched_barrier(0);
+        load(0, d0, f0);  // (without steps too: a wait for the query does not wait for these then)
+        __builtin_amdgcn_sched_barrier(0);
+
+        float cs = fminf(fabsf(a.scale) * 1.44269504088896341f, FLT_MAX);
+        const float sign = a.scale < 0.f ? -1.f : a.scale > 0.f ? 1.f : 0.f;
+        typedef std::conditional_t<H16, half8, floatx4> qvec;
+        qvec qf[QP][KS];
+        if constexpr (QP == 2) {
+            float top = 0.f;
+#pragma unroll
+            for (int s = 0; s < KS; s++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(__builtin_bit_cast(floatx4, qw[s][i / 4])[i % 4]));
+            top = lane_pair_max<16>(top);
+            top = lane_pair_max<32>(top);
+            // the row's largest entry to 2^14 .. 2^15
+            const int up = top > 0.f && top <= FLT_MAX ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
+            cs = fminf(ldexpf(fabsf(a.scale) * 1.44269504088896341f, -up), FLT_MAX);
+#pragma unroll
+            for (int s = 0; s < KS; s++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float f = ldexpf(__builtin_bit_cast(floatx4, qw[s][i / 4])[i % 4] * sign, up);
+                    qf[0][s][i] = (_Float16)f;
+                    qf[1][s][i] = (_Float16)(f - (float)qf[0][s][i]);
+                }
+        } else {
+#pragma unroll
+            for (int s = 0; s < KS; s++)
+#pragma unroll
+                for (int i = 0; i < L::PIECE; i++) qf[0][s][i] = __builtin_bit_cast(qvec, qw[s][0])[i] * (QT)sign;
+        }
+        cs = fmaxf(cs, FLT_MIN);
+
         float m = -INFINITY, l = 0.f;
         floatx4 acc[NA];
 #pragma unroll
@@ -413,28 +437,26 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_tile(
             }
         };
 
+        // the next block's loads are in flight under this one's work; no load is conditional
+        // inside the loop, or the waits would count for the path without it
         if (steps > 0) {
-            Buf f0, f1;
-            Ids d0 = ids_of(0), d1 = d0;
-            load(0, d0, f0);
-            if (steps > 1) d1 = ids_of(1);
-            for (int s = 0; s < steps; s += 2) {
-                if (s + 1 < steps) load(s + 1, d1, f1);
+            int s = 0;
+            for (; s + 2 < steps; s += 2) {
+                load(s + 1, d1, f1);
                 __builtin_amdgcn_sched_barrier(0);
-                Ids d2 = d0;
-                if (s + 2 < steps) d2 = ids_of(s + 2);
+                const Ids d2 = ids_of(s + 2), d3 = ids_of(min(s + 3, steps - 1));
                 compute(s, d0, f0);
                 __builtin_amdgcn_sched_barrier(0);
-                if (s + 1 >= steps) break;
-                if (s + 2 < steps) load(s + 2, d2, f0);
+                load(s + 2, d2, f0);
                 __builtin_amdgcn_sched_barrier(0);
-                d0 = d2;
-                Ids d3 = d1;
-                if (s + 3 < steps) d3 = ids_of(s + 3);
                 compute(s + 1, d1, f1);
                 __builtin_amdgcn_sched_barrier(0);
-                d1 = d3;
+                d0 = d2, d1 = d3;
             }
+            if (s + 1 < steps) load(s + 1, d1, f1);
+            __builtin_amdgcn_sched_barrier(0);
+            compute(s, d0, f0);
+            if (s + 1 < steps) compute(s + 1, d1, f1);
         }
         l = lane_pair_sum<16>(l);
         l = lane_pair_sum<32>(l);
@@ -463,9 +485,9 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_tile(
         const bool whole = r0 == 0 && r1 == w.rounds;
         const int orow = tile * 16 + tr, oq = orow / G;
         float* rec = a.ws + (int64_t)(2 * run + (r0 == 0 ? 1 : 0)) * 16 * (D + 4) + tr * (D + 4);
-        const int64_t sees = shown + oq;
-        const float inv = sees > len ? NAN : 1.0f / sum;
-        QT* op = static_cast<QT*>(a.out) + ((int64_t)(first + oq) * a.hq + h * G + orow - oq * G) * D;
+        const int sees = sq.shown + oq;
+        const float inv = sees > sq.len ? NAN : 1.0f / sum;
+        QT* op = static_cast<QT*>(a.out) + ((int64_t)(sq.first + oq) * a.hq + h * G + orow - oq * G) * D;
         if (orow < rows) {
 #pragma unroll
             for (int i = 0; i < (DP + 63) / 64; i++) {
@@ -516,7 +538,8 @@ typedef short short4v __attribute__((ext_vector_type(4)));
 
 template <typename QT, int DP>
 __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_prompt(
-    const PagedAttn a, const int32_t* __restrict__ table, const char* __restrict__ kp, const char* __restrict__ vp) {
+    const PagedAttn a, const int32_t* __restrict__ table, const int32_t* __restrict__ cu, const int32_t* __restrict__ lens,
+    const char* __restrict__ kp, const char* __restrict__ vp) {
     using L = PromptTile<DP>;
     constexpr int KT = L::KT, CPR = L::CPR, U = L::U, RPW = KT / 4;
     constexpr int QP = std::is_same_v<QT, float> ? 2 : 1;  // f16 parts of a query, and of a weight
@@ -531,13 +554,11 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_prompt(
 
     // tiles from the last one back: of one sequence the longest first
     const int h = blockIdx.x % c.hkv, back = blockIdx.x / c.hkv;
-    auto tiles_of = [&](int b) {
-        int f;
-        return b < c.batch ? (paged_rows(c, b, &f) * G + 127) >> 7 : 0;
-    };
+    Group grp;
     int64_t total = 0, incl = 0, mine = 0;
     for (int base = 0; base < c.batch; base += 64) {
-        mine = tiles_of(base + lane);
+        grp.load(c, cu, lens, base);
+        mine = (grp.q.n * G + 127) >> 7;
         incl = lane_prefix(mine);
         total += lane_value(incl, 63);
     }
@@ -547,7 +568,8 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_prompt(
     int64_t before = 0;
     for (int base = 0;; base += 64) {
         if (c.batch > 64) {
-            mine = tiles_of(base + lane);
+            grp.load(c, cu, lens, base);
+            mine = (grp.q.n * G + 127) >> 7;
             incl = lane_prefix(mine);
         }
         const uint64_t hit = __ballot(nth < before + incl);
@@ -559,14 +581,9 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_prompt(
         }
         before += lane_value(incl, 63);
     }
-    b = __builtin_amdgcn_readfirstlane(b);
-    tile = __builtin_amdgcn_readfirstlane(tile);
-
-    int first;
-    bool past;
-    const int n = paged_rows(c, b, &first), len = paged_len(c, b, &past), rows = n * G;
-    const int64_t shown = (int64_t)max(c.lens[b], 0) - n + 1;  // positions that query 0 sees
-    auto limit = [&](int row) { return (int)max(min(shown + min(row, rows - 1) / G, (int64_t)len), (int64_t)0); };
+    const Seq sq = grp.at(b);
+    const int rows = sq.n * G;
+    auto limit = [&](int row) { return limit_of(sq, min(row, rows - 1) / G); };
     auto uniform = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
     const int w0 = tile * 128 + wave * 32, r = min(w0 + col, rows - 1), qi = r / G, qh = h * G + r - qi * G;
     const int lim = limit(r), lim_hi = uniform(limit(w0 + 31));
@@ -574,7 +591,7 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_prompt(
     const bool live = w0 < rows;
 
     // this lane's part of its row: dimensions 16 s + 8 hf ..
-    const QT* qp = static_cast<const QT*>(a.q) + (int64_t)(first + qi) * a.q_stride + qh * D;
+    const QT* qp = static_cast<const QT*>(a.q) + (int64_t)(sq.first + qi) * a.q_stride + qh * D;
     const float sign = a.scale < 0.f ? -1.f : a.scale > 0.f ? 1.f : 0.f;
     float cs = fminf(fabsf(a.scale) * 1.44269504088896341f, FLT_MAX);
     half8 qf[QP][KS];
@@ -767,9 +784,9 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_prompt(
     }
     l = lane_pair_sum<32>(l);
     if (w0 + col >= rows) return;
-    const int64_t sees = shown + qi;
-    const float inv = sees > len ? NAN : 1.0f / l;
-    QT* op = static_cast<QT*>(a.out) + ((int64_t)(first + qi) * a.hq + qh) * D;
+    const int sees = sq.shown + qi;
+    const float inv = sees > sq.len ? NAN : 1.0f / l;
+    QT* op = static_cast<QT*>(a.out) + ((int64_t)(sq.first + qi) * a.hq + qh) * D;
 #pragma unroll
     for (int i = 0; i < DT; i++)
 #pragma unroll
@@ -787,19 +804,24 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_prompt(
 // Tiles that several runs share, and those without a position: one workgroup per (sequence, KV
 // head, tile) that there can be, in the line's order.
 template <typename QT>
-__global__ __launch_bounds__(256) void k_paged_join(const PagedAttn a, int keys, int runs) {
+__global__ __launch_bounds__(256) void k_paged_join(const PagedAttn a, const int32_t* __restrict__ cu, const int32_t* __restrict__ lens, int keys, int runs) {
+    __shared__ float weight[16][RUNS], total_of[16];
+    __shared__ floatx4 partial[256];
     const PagedCache& c = a.c;
-    const int lane = threadIdx.x & 63, G = a.G, D = c.D;
+    const int G = a.G, D = c.D;
+    Group grp;
+    Seq sq{};
     int64_t total = 0, units = 0, at = -1, nth = 0;
     int b = -1;
     for (int base = 0; base < c.batch; base += 64) {
-        Work w{0, 0};
-        if (base + lane < c.batch) w = work_of(c, base + lane, G, keys);
+        grp.load(c, cu, lens, base);
+        const Work w = work_of(grp.q, G, keys);
         const int64_t wu = (int64_t)c.hkv * w.tiles, ww = wu * w.rounds, iu = lane_prefix(wu), iw = lane_prefix(ww);
         const uint64_t hit = __ballot(blockIdx.x < units + iu);
         if (b < 0 && hit) {
             const int i = __builtin_ctzll(hit);
             b = base + i;
+            sq = grp.at(b);
             nth = blockIdx.x - (units + lane_value(iu, i) - lane_value(wu, i));
             at = total + lane_value(iw, i) - lane_value(ww, i);
         }
@@ -807,50 +829,74 @@ __global__ __launch_bounds__(256) void k_paged_join(const PagedAttn a, int keys,
         total += lane_value(iw, 63);
     }
     if (b < 0) return;
-    const Work w = work_of(c, b, G, keys);
+    const Work w = work_of(sq, G, keys);
     const int64_t len_run = total <= runs ? 1 : (total + runs - 1) / runs;
     const int64_t x = at + nth * w.rounds;
     const int64_t run0 = x / len_run, run1 = w.rounds ? (x + w.rounds - 1) / len_run : run0;
     if (w.rounds && run0 == run1) return;
     const int h = (int)(nth / w.tiles), tile = (int)(nth - (int64_t)h * w.tiles);
-    int first;
-    bool past;
-    const int n = paged_rows(c, b, &first), len = paged_len(c, b, &past), rows = n * G;
-    const int tr = threadIdx.x >> 4, tc = threadIdx.x & 15, orow = tile * 16 + tr, oq = orow / G;
-    if (orow >= rows) return;
-    const int64_t sees = (int64_t)max(c.lens[b], 0) - n + 1 + oq;
-    const float* rec = a.ws + (2 * run0 + 1) * 16 * (D + 4) + tr * (D + 4);  // the next ones: slot 0 of run0 + 1, ...
-    const int64_t step = (int64_t)2 * 16 * (D + 4);
-    const int parts = w.rounds ? (int)(run1 - run0 + 1) : 0;
-    auto part = [&](int i) { return i == 0 ? rec : rec + i * step - 16 * (D + 4); };
-    float M = -INFINITY;
-    for (int i = 0; i < parts; i++) M = fmaxf(M, part(i)[D]);
-    const float Ms = M == -INFINITY ? 0.f : M;
-    floatx4 o[4] = {};
-    float sum = 0.f;
-    for (int i = 0; i < parts; i++) {
-        const float* p = part(i);
-        const floatx4 mlc = *reinterpret_cast<const floatx4*>(p + D);
-        const float f = __builtin_amdgcn_exp2f((mlc[0] - Ms) * mlc[2]);
-        sum = fmaf(mlc[1], f, sum);
+    const int parts = w.rounds ? (int)(run1 - run0 + 1) : 0, R = min(16, sq.n * G - tile * 16), per = D / 4;
+    const float* rec = a.ws + (2 * run0 + 1) * 16 * (D + 4);  // then slot 0 of run0 + 1, run0 + 2, ...
+    auto part = [&](int i) { return i == 0 ? rec : rec + (2 * i - 1) * (int64_t)(16 * (D + 4)); };
+    // the parts' weights: a wavefront per row, a lane per part
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int r = wave; r < R; r += 4) {
+        float m[RUNS / 64], l[RUNS / 64], cs = 0.f, M = -INFINITY;
 #pragma unroll
-        for (int u = 0; u < 4; u++)
-            if (64 * u + 4 * tc < D) {
-                const floatx4 z = *reinterpret_cast<const floatx4*>(p + 64 * u + 4 * tc);
-#pragma unroll
-                for (int e = 0; e < 4; e++) o[u][e] = fmaf(z[e], f, o[u][e]);
+        for (int i = 0; i < RUNS / 64; i++) {
+            m[i] = -INFINITY, l[i] = 0.f;
+            if (64 * i + lane < parts) {
+                const floatx4 z = *reinterpret_cast<const floatx4*>(part(64 * i + lane) + r * (D + 4) + D);
+                m[i] = z[0], l[i] = z[1], cs = z[2];
             }
-    }
-    const float inv = sees > len ? NAN : 1.0f / sum;
-    QT* op = static_cast<QT*>(a.out) + ((int64_t)(first + oq) * a.hq + h * G + orow - oq * G) * D;
+            M = fmaxf(M, m[i]);
+        }
+        M = wave_allmax(M);
+        cs = wave_allmax(cs);  // one value for all parts, at least FLT_MIN
+        const float Ms = M == -INFINITY ? 0.f : M;
+        float sum = 0.f;
 #pragma unroll
-    for (int u = 0; u < 4; u++) {
-        const int dim = 64 * u + 4 * tc;
-        if (dim >= D) break;
-        const floatx4 v = sees <= 0 ? floatx4{0.f, 0.f, 0.f, 0.f} : o[u] * inv;
-        if constexpr (std::is_same_v<QT, float>) *reinterpret_cast<floatx4*>(op + dim) = v;
-        else *reinterpret_cast<half4v*>(op + dim) = half4v{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
+        for (int i = 0; i < RUNS / 64; i++)
+            if (64 * i + lane < parts) {
+                const float f = __builtin_amdgcn_exp2f((m[i] - Ms) * cs);
+                sum = fmaf(l[i], f, sum);
+                weight[r][64 * i + lane] = f;
+            }
+        sum = wave_allsum(sum);
+        if (lane == 0) total_of[r] = sum;
     }
+    __syncthreads();
+    // few rows: the parts in slices, added in order
+    const int items = R * per, slices = max(256 / items, 1);
+    auto put = [&](int it, floatx4 o) {
+        const int r = it / per, dim = 4 * (it - r * per), orow = tile * 16 + r, oq = orow / G, sees = sq.shown + oq;
+        o *= sees > sq.len ? NAN : 1.0f / total_of[r];
+        if (sees <= 0) o = floatx4{0.f, 0.f, 0.f, 0.f};
+        QT* op = static_cast<QT*>(a.out) + ((int64_t)(sq.first + oq) * a.hq + h * G + orow - oq * G) * D;
+        if constexpr (std::is_same_v<QT, float>) *reinterpret_cast<floatx4*>(op + dim) = o;
+        else *reinterpret_cast<half4v*>(op + dim) = half4v{(_Float16)o[0], (_Float16)o[1], (_Float16)o[2], (_Float16)o[3]};
+    };
+    const int slice = slices > 1 ? (int)threadIdx.x / items : 0;
+    for (int it = slices > 1 ? (int)threadIdx.x - slice * items : (int)threadIdx.x; it < items; it += 256) {
+        if (slice >= slices) break;
+        const int r = it / per, at4 = r * (D + 4) + 4 * (it - r * per);
+        floatx4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+        for (int i = slice; i < parts; i += slices) {
+            const floatx4 z = *reinterpret_cast<const floatx4*>(part(i) + at4);
+            const float f = weight[r][i];
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[e] = fmaf(z[e], f, o[e]);
+        }
+        if (slices == 1) put(it, o);
+        else partial[threadIdx.x] = o;
+    }
+    if (slices == 1) return;
+    __syncthreads();
+    if ((int)threadIdx.x >= items) return;
+    floatx4 o = partial[threadIdx.x];
+    for (int i = 1; i < slices; i++) o += partial[threadIdx.x + i * items];
+    put(threadIdx.x, o);
 }
 
 size_t paged_attention_workspace(int64_t batch, int64_t rows, int hq, int hkv, int D) {
@@ -864,8 +910,8 @@ static int launch_tile_of(const PagedAttn& a, hipStream_t s) {
     const int64_t units = a.c.hkv * (a.c.cu ? cdiv((int64_t)a.c.rows * a.G, 16) + a.c.batch : (int64_t)a.c.batch * cdiv(a.G, 16));
     const int64_t most = units * cdiv(a.c.capacity, KEYS);
     const int runs = (int)(most < RUNS ? most : RUNS);
-    k_paged_tile<KVT, QT, DP, TK, FULL><<<dim3((unsigned)runs), 256, 0, s>>>(a, a.c.table, static_cast<const char*>(a.c.k), static_cast<const char*>(a.c.v));
-    k_paged_join<QT><<<dim3((unsigned)units), 256, 0, s>>>(a, KEYS, runs);
+    k_paged_tile<KVT, QT, DP, TK, FULL><<<dim3((unsigned)runs), 256, 0, s>>>(a, a.c.table, a.c.cu, a.c.lens, static_cast<const char*>(a.c.k), static_cast<const char*>(a.c.v));
+    k_paged_join<QT><<<dim3((unsigned)units), 256, 0, s>>>(a, a.c.cu, a.c.lens, KEYS, runs);
     hipError_t e = hipGetLastError();
     return e == hipSuccess ? TL_HIP_OK : hip_fail(e, "paged attention launch");
 }
@@ -878,7 +924,7 @@ static int launch_tile(const PagedAttn& a, hipStream_t s) {
 template <typename QT, int DP>
 static int launch_prompt(const PagedAttn& a, hipStream_t s) {
     const int64_t units = a.c.hkv * (cdiv((int64_t)a.c.rows * a.G, 128) + a.c.batch);
-    k_paged_prompt<QT, DP><<<dim3((unsigned)units), 256, 0, s>>>(a, a.c.table, static_cast<const char*>(a.c.k), static_cast<const char*>(a.c.v));
+    k_paged_prompt<QT, DP><<<dim3((unsigned)units), 256, 0, s>>>(a, a.c.table, a.c.cu, a.c.lens, static_cast<const char*>(a.c.k), static_cast<const char*>(a.c.v));
     hipError_t e = hipGetLastError();
     return e == hipSuccess ? TL_HIP_OK : hip_fail(e, "paged attention launch");
 }
