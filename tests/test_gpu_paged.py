@@ -303,6 +303,31 @@ def test_lens_and_splits_repeat_themselves(dev):
     assert np.array_equal(run_attention(s, qp, 0.09, cu=[0, 4, 6], upload=False), first)
 
 
+@pytest.mark.parametrize("qt,kt", TYPES)
+def test_parts_joined_in_the_same_launch_or_after_it(dev, qt, kt):
+    """The two forms give the same bits: long and short sequences, empty ones, more rows than one
+    tile holds."""
+    lib = _lib.load()
+    lens = [9000, 0, 3, 700, 1, 0, 2500]
+    s = Setup(dev, 25, lens, 64, 2, 128, kt)
+    q = s.rng.standard_normal((len(lens), 40, 128)).astype(qt)
+    new = [5, 0, 3, 40, 1, 7, 2]
+    cu = np.concatenate([[0], np.cumsum(new)])
+    qp = s.rng.standard_normal((cu[-1], 40, 128)).astype(qt)
+    got = {}
+    was = lib.tl_hip_debug_one_launch_merge(-1)
+    for form in (0, 1):
+        before = lib.tl_hip_debug_one_launch_merge(form)
+        try:
+            got[form] = run_attention(s, q, 0.09), run_attention(s, qp, 0.09, cu=cu)
+        finally:
+            lib.tl_hip_debug_one_launch_merge(before)
+    check(got[0][0], *attention(q, s.k, s.v, s.table, lens, range(8), 64, 0.09, qt == np.float16))
+    check(got[0][1], *attention(qp, s.k, s.v, s.table, lens, cu, 64, 0.09, qt == np.float16))
+    assert np.array_equal(got[0][0], got[1][0]) and np.array_equal(got[0][1], got[1][1])
+    assert lib.tl_hip_debug_one_launch_merge(-1) == was
+
+
 def test_offsets_past_32_bits(dev):
     """Pools past 4 GiB each: the pages in use lie at their far end."""
     lib = _lib.load()

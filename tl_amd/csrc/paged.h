@@ -42,6 +42,7 @@ struct PagedAttn {
     int32_t hq, G;
     float scale;
     float* ws;
+    bool fuse;  // parts may be joined in the launch that made them: no other call overlaps
 };
 // q and out are f16 (q16) or f32, the cache f16 (kv16) or f32; not q16 over an f32 cache.
 int launch_paged_attention(const PagedAttn& a, bool q16, bool kv16, hipStream_t s);

@@ -141,6 +141,8 @@ static int attend(PagedAttn a, int q_dtype, int kv_dtype, void* workspace, size_
     void* ws = workspace ? workspace : dev_alloc_on(need, on.s);
     if (!ws) return TL_HIP_ERR_ALLOC;
     a.ws = static_cast<float*>(ws);
+    // the arrival counters are the device's: only while calls cannot overlap, and not in a graph
+    a.fuse = single_stream() && one_launch_merge() && !on.capturing;
     const int rc = launch_paged_attention(a, q_dtype == TL_HIP_F16, kv_dtype == TL_HIP_F16, on.s);
     if (!workspace) dev_free_on(ws, on.s);
     return rc;

@@ -37,9 +37,9 @@ struct Group {
         const int b = from + (int)__lane_id();
         q = Seq{0, 0, 0, 0};
         if (b >= c.batch) return;
-        int lo = b, hi = b + 1;
-        if (cu) lo = min(max(cu[b], 0), c.rows), hi = min(max(cu[b + 1], 0), c.rows);
-        const int n = min(max(lens[b], 0), INT32_MAX - 32);
+        int n = lens[b], lo = b, hi = b + 1;  // (requested together)
+        if (cu) lo = cu[b], hi = cu[b + 1];
+        lo = min(max(lo, 0), c.rows), hi = min(max(hi, 0), c.rows), n = min(max(n, 0), INT32_MAX - 32);
         q.first = lo, q.n = max(hi - lo, 0), q.len = min(n, c.capacity), q.shown = n - q.n + 1;
     }
     __device__ __forceinline__ Seq at(int b) const {
@@ -76,6 +76,9 @@ __device__ __forceinline__ int64_t lane_prefix(int64_t v) {
     }
     return v;
 }
+__device__ __forceinline__ int64_t run_length(int64_t total, int runs) {
+    return total <= runs ? 1 : total <= 0x7FFFFFFF ? ((uint32_t)total + runs - 1) / (uint32_t)runs : (total + runs - 1) / runs;
+}
 __device__ __forceinline__ uint32_t div_u(int64_t a, int64_t b) {
     if (((a | b) >> 32) == 0) return (uint32_t)a / (uint32_t)b;
     return (uint32_t)((uint64_t)a / (uint64_t)b);
@@ -88,6 +91,80 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
     const uint32_t top = ((w & 0x7C007C00u) + 0x04000400u) & 0x80008000u;  // the exponent's carry
     return (top - (top >> 15)) | top;
 }
+
+// Adds the parts of a tile that runs run0 .. run0 + parts - 1 left, in order, and writes its rows:
+// a thread per four elements, over all parts or, where the rows are few, over every `slices`-th
+// and then over the slices.  Eight parts are requested at a time.
+constexpr int JOIN_ROOM = 256 * 7;  // floats of LDS
+template <typename QT, int POLICY>
+__device__ __forceinline__ void join_tile(const PagedAttn& a, const Seq& sq, int h, int tile, int run0, int parts, float* room) {
+    const int G = a.G, D = a.c.D, R = min(16, sq.n * G - tile * 16), per = D / 4;
+    const uint32_t rec = 16 * (D + 4) * 4, row = (D + 4) * 4;  // bytes
+    const __amdgpu_buffer_rsrc_t ws = buf_rsrc(a.ws, RUNS * 2 * rec);
+    auto part = [&](int i) { return (uint32_t)(2 * (run0 + i) + (i == 0 ? 1 : 0)) * rec; };  // the first in slot 1, the rest in slot 0
+    auto word4 = [&](uint32_t at) { return __builtin_bit_cast(floatx4, __builtin_amdgcn_raw_buffer_load_b128(ws, at, 0, POLICY)); };
+    floatx4* po = reinterpret_cast<floatx4*>(room);
+    float *pm = room + 1024, *pl = room + 1280;
+    struct Sum {
+        floatx4 o;
+        float m, l, cs;
+    };
+    auto add = [](Sum& t, const floatx4& o, float m, float l) {
+        const float mn = fmaxf(t.m, m), ms = mn == -INFINITY ? 0.f : mn;
+        const float f = __builtin_amdgcn_exp2f((t.m - ms) * t.cs), g = __builtin_amdgcn_exp2f((m - ms) * t.cs);
+        t.m = mn;
+        t.l = fmaf(t.l, f, l * g);
+#pragma unroll
+        for (int e = 0; e < 4; e++) t.o[e] = fmaf(t.o[e], f, o[e] * g);
+    };
+    const int items = R * per, slices = max(256 / items, 1);
+    auto put = [&](int it, const Sum& t) {
+        const int r = it / per, dim = 4 * (it - r * per), orow = tile * 16 + r, oq = orow / G, sees = sq.shown + oq;
+        floatx4 o = t.o * (sees > sq.len ? NAN : 1.0f / t.l);
+        if (sees <= 0) o = floatx4{0.f, 0.f, 0.f, 0.f};
+        QT* op = static_cast<QT*>(a.out) + ((int64_t)(sq.first + oq) * a.hq + h * G + orow - oq * G) * D;
+        if constexpr (std::is_same_v<QT, float>) *reinterpret_cast<floatx4*>(op + dim) = o;
+        else *reinterpret_cast<half4v*>(op + dim) = half4v{(_Float16)o[0], (_Float16)o[1], (_Float16)o[2], (_Float16)o[3]};
+    };
+    const int slice = slices > 1 ? (int)threadIdx.x / items : 0;
+    for (int it = slices > 1 ? (int)threadIdx.x - slice * items : (int)threadIdx.x; it < items && slice < slices; it += 256) {
+        const int r = it / per;
+        Sum t{{0.f, 0.f, 0.f, 0.f}, -INFINITY, 0.f, 1.f};
+        for (int i0 = slice; i0 < parts; i0 += 8 * slices) {
+            floatx4 z[8], ml[8];
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                // (an offset at the resource's end reads nothing)
+                const uint32_t at = i0 + u * slices < parts ? part(i0 + u * slices) + r * row : RUNS * 2 * rec;
+                z[u] = word4(at + 16 * (it - r * per));
+                ml[u] = word4(at + 4 * D);
+            }
+#pragma unroll
+            for (int u = 0; u < 8; u++)
+                if (i0 + u * slices < parts) {
+                    t.cs = ml[u][2];  // one value for all parts
+                    add(t, z[u], ml[u][0], ml[u][1]);
+                }
+        }
+        if (slices == 1) {
+            put(it, t);
+        } else {
+            po[threadIdx.x] = t.o, pm[threadIdx.x] = t.m, pl[threadIdx.x] = t.l;
+            if (slice == 0) room[1536 + threadIdx.x] = t.cs;
+        }
+    }
+    if (slices == 1) return;
+    __syncthreads();
+    const int it = threadIdx.x;
+    if (it >= items) return;
+    Sum t{po[it], pm[it], pl[it], room[1536 + it]};
+    for (int i = 1; i < slices; i++)
+        if (i < parts) add(t, po[it + i * items], pm[it + i * items], pl[it + i * items]);
+    put(it, t);
+}
+// One launch: arrivals at the tile that run `i` began, zero between calls.  The run that arrives
+// last joins the tile and sets its counter back.
+__device__ uint32_t g_paged_arrive[RUNS];
 
 // ---- 16 rows, keys and values straight from memory into matrix operands ------------------
 // A wavefront takes 16 TK positions of a round at a time, the four wavefronts of a workgroup
@@ -127,9 +204,15 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_tile(
     typedef uint32_t words __attribute__((ext_vector_type(sizeof(vec) / 4)));
     typedef KVT piece __attribute__((ext_vector_type(L::PIECE)));
     constexpr int RS = DP + 4;
-    __shared__ __attribute__((aligned(16))) float so[4][16][RS];  // o, then m and l
+    __shared__ __attribute__((aligned(16))) float so[4][16][RS];  // o, then m, l and c
+    __shared__ int last_here;
+    static_assert(sizeof(so) >= JOIN_ROOM * 4, "the join's room");
     const PagedCache& c = a.c;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
+    // arguments in one round of scalar loads (left to the compiler: three dependent rounds)
+    asm volatile("" : : "s"(table), "s"(cu), "s"(lens), "s"(kp), "s"(vp), "s"(a.q), "s"(a.out), "s"(a.q_stride), "s"(a.hq), "s"(a.G),
+                 "s"(a.scale), "s"(c.table_stride), "s"(c.page_elems), "s"(c.n_pages), "s"(c.batch), "s"(c.rows), "s"(c.hkv),
+                 "s"(c.D), "s"(c.shift), "s"(c.capacity));
     const int G = a.G, D = FULL ? DP : c.D, page = 1 << c.shift;
     // run: neighbours on the line stay on one XCD (workgroups go round the eight of them)
     const int runs = gridDim.x, id = blockIdx.x;
@@ -143,8 +226,17 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_tile(
         mine = (int64_t)c.hkv * w.tiles * w.rounds;
         incl = lane_prefix(mine);
         total += lane_value(incl, 63);
+        // rows of sequences without a position are zeros, and no round's
+        for (uint64_t none = __ballot(w.tiles > 0 && w.rounds == 0); none; none &= none - 1) {
+            const int i = __builtin_ctzll(none);
+            if ((base + i) % runs != run) continue;
+            const Seq sq = grp.at(base + i);
+            uint32_t* op = reinterpret_cast<uint32_t*>(static_cast<QT*>(a.out) + (int64_t)sq.first * a.hq * D);
+            const int64_t words = (int64_t)sq.n * a.hq * D * (int)sizeof(QT) / 4;
+            for (int64_t u = threadIdx.x; u < words; u += 256) op[u] = 0;
+        }
     }
-    const int64_t len_run = total <= runs ? 1 : total <= 0x7FFFFFFF ? ((uint32_t)total + runs - 1) / (uint32_t)runs : (total + runs - 1) / runs;
+    const int64_t len_run = run_length(total, runs);
     int64_t x = run * len_run;
     const int64_t x1 = min(x + len_run, total);
     if (x >= x1) return;
@@ -180,6 +272,7 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_tile(
         const int r0 = __builtin_amdgcn_readfirstlane((int)(x - before - (int64_t)unit * w.rounds));
         const int r1 = __builtin_amdgcn_readfirstlane((int)min((int64_t)w.rounds, r0 + (x1 - x)));
         const int h = unit / w.tiles, tile = unit - h * w.tiles;
+        const int64_t begin = x - r0;
         x += r1 - r0;
 
         // this lane's row; positions that it, that every row and that any row sees
@@ -484,7 +577,8 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_tile(
         for (int v = 0; v < 4; v++) fw[v] = __builtin_amdgcn_exp2f((so[v][tr][DP] - Ms) * rc), sum = fmaf(so[v][tr][DP + 1], fw[v], sum);
         const bool whole = r0 == 0 && r1 == w.rounds;
         const int orow = tile * 16 + tr, oq = orow / G;
-        float* rec = a.ws + (int64_t)(2 * run + (r0 == 0 ? 1 : 0)) * 16 * (D + 4) + tr * (D + 4);
+        const uint32_t rec = (uint32_t)(2 * run + (r0 == 0 ? 1 : 0)) * (16 * (D + 4) * 4) + tr * (D + 4) * 4;  // bytes
+        const __amdgpu_buffer_rsrc_t ws = buf_rsrc(a.ws, RUNS * 2 * 16 * (D + 4) * 4);
         const int sees = sq.shown + oq;
         const float inv = sees > sq.len ? NAN : 1.0f / sum;
         QT* op = static_cast<QT*>(a.out) + ((int64_t)(sq.first + oq) * a.hq + h * G + orow - oq * G) * D;
@@ -501,7 +595,8 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_tile(
                     for (int e = 0; e < 4; e++) o[e] = fmaf(z[e], fw[v], o[e]);
                 }
                 if (!whole) {
-                    *reinterpret_cast<floatx4*>(rec + dim) = o;
+                    // through to where every XCD sees it
+                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), ws, rec + 4 * dim, 0, CPOL_SC1);
                 } else {
                     if (sees <= 0) o = floatx4{0.f, 0.f, 0.f, 0.f};
                     else o *= inv;
@@ -509,9 +604,62 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_tile(
                     else *reinterpret_cast<half4v*>(op + dim) = half4v{(_Float16)o[0], (_Float16)o[1], (_Float16)o[2], (_Float16)o[3]};
                 }
             }
-            if (!whole && tc == 0) *reinterpret_cast<floatx4*>(rec + D) = floatx4{M, sum, rc, 0.f};
+            if (!whole && tc == 0)
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, floatx4{M, sum, rc, 0.f}), ws, rec + 4 * D, 0, CPOL_SC1);
+        }
+        if (a.fuse && !whole) {
+            // Every wave waits until its record has reached the point that all XCDs see, then
+            // one thread arrives; the records are read past the caches, after the arrival.
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            const int run0 = (int)div_u(begin, len_run), parts = (int)div_u(begin + w.rounds - 1, len_run) - run0 + 1;
+            if (threadIdx.x == 0) {
+                const uint32_t old = __hip_atomic_fetch_add(&g_paged_arrive[run0], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                const bool end = old == (uint32_t)(parts - 1);
+                if (end) __hip_atomic_store(&g_paged_arrive[run0], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                last_here = end;
+            }
+            __syncthreads();
+            if (last_here) join_tile<QT, CPOL_SC1>(a, sq, h, tile, run0, parts, &so[0][0][0]);
         }
     }
+}
+
+// The tile of 2^shift rows that a workgroup of the prompt kernels takes: KV heads next to each
+// other (on XCDs of their own), tiles from the last one back, so that of one sequence the longest
+// come first.
+__device__ __forceinline__ bool prompt_tile(const PagedCache& c, const int32_t* cu, const int32_t* lens, int G, int shift, Seq* sq,
+                                            int* b, int* h, int* tile) {
+    *h = blockIdx.x % c.hkv;
+    const int back = blockIdx.x / c.hkv, up = (1 << shift) - 1;
+    Group grp;
+    int64_t total = 0, incl = 0, mine = 0;
+    for (int base = 0; base < c.batch; base += 64) {
+        grp.load(c, cu, lens, base);
+        mine = (grp.q.n * G + up) >> shift;
+        incl = lane_prefix(mine);
+        total += lane_value(incl, 63);
+    }
+    const int64_t nth = total - 1 - back;
+    if (nth < 0) return false;
+    int64_t before = 0;
+    for (int base = 0;; base += 64) {
+        if (c.batch > 64) {
+            grp.load(c, cu, lens, base);
+            mine = (grp.q.n * G + up) >> shift;
+            incl = lane_prefix(mine);
+        }
+        const uint64_t hit = __ballot(nth < before + incl);
+        if (hit) {
+            const int at = __builtin_ctzll(hit);
+            *b = base + at;
+            *tile = __builtin_amdgcn_readfirstlane((int)(nth - (before + lane_value(incl, at) - lane_value(mine, at))));
+            break;
+        }
+        before += lane_value(incl, 63);
+    }
+    *sq = grp.at(*b);
+    return true;
 }
 
 // ---- prompts over f16 caches -------------------------------------------------------------
@@ -552,36 +700,9 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_prompt(
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, hf = lane >> 5;
     const int G = a.G, D = c.D, page = 1 << c.shift;
 
-    // tiles from the last one back: of one sequence the longest first
-    const int h = blockIdx.x % c.hkv, back = blockIdx.x / c.hkv;
-    Group grp;
-    int64_t total = 0, incl = 0, mine = 0;
-    for (int base = 0; base < c.batch; base += 64) {
-        grp.load(c, cu, lens, base);
-        mine = (grp.q.n * G + 127) >> 7;
-        incl = lane_prefix(mine);
-        total += lane_value(incl, 63);
-    }
-    const int64_t nth = total - 1 - back;
-    if (nth < 0) return;
-    int b = 0, tile = 0;
-    int64_t before = 0;
-    for (int base = 0;; base += 64) {
-        if (c.batch > 64) {
-            grp.load(c, cu, lens, base);
-            mine = (grp.q.n * G + 127) >> 7;
-            incl = lane_prefix(mine);
-        }
-        const uint64_t hit = __ballot(nth < before + incl);
-        if (hit) {
-            const int at = __builtin_ctzll(hit);
-            b = base + at;
-            tile = (int)(nth - (before + lane_value(incl, at) - lane_value(mine, at)));
-            break;
-        }
-        before += lane_value(incl, 63);
-    }
-    const Seq sq = grp.at(b);
+    Seq sq;
+    int b, h, tile;
+    if (!prompt_tile(c, cu, lens, G, 7, &sq, &b, &h, &tile)) return;
     const int rows = sq.n * G;
     auto limit = [&](int row) { return limit_of(sq, min(row, rows - 1) / G); };
     auto uniform = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
@@ -639,7 +760,7 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_prompt(
     }
     const int32_t* row = table + (int64_t)b * c.table_stride;
     const int64_t head = (int64_t)h * page * D;
-    auto page_of = [&](int j0) { return __builtin_amdgcn_readfirstlane(row[min(j0 + wave * RPW, last - 1) >> c.shift]); };
+    auto page_of = [&](int j0) { return uniform(row[max(min(j0 + wave * RPW, last - 1), 0) >> c.shift]); };
     auto issue = [&](int j0, int pid, Stage& st) __attribute__((always_inline)) {
         const int j = j0 + wave * RPW;
         const bool none = (uint32_t)pid >= (uint32_t)c.n_pages;
@@ -801,14 +922,199 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_prompt(
         }
 }
 
-// Tiles that several runs share, and those without a position: one workgroup per (sequence, KV
-// head, tile) that there can be, in the line's order.
+// ---- prompts over f32 caches -------------------------------------------------------------
+// The same with f32 matrix instructions (v_mfma_f32_16x16x4_f32): 64 rows to a workgroup, 16 to a
+// wavefront, 16 KiB of keys and of values at a time.  Lane (col, g) holds row col's scores at
+// keys 4 g + e of 16; one 16-byte read of a value row feeds four matrix instructions, dimension
+// 64 j + 4 r + y in row r of number y.
+template <int DP>
+__global__ __launch_bounds__(256, 2) void k_paged_prompt_f32(
+    const PagedAttn a, const int32_t* __restrict__ table, const int32_t* __restrict__ cu, const int32_t* __restrict__ lens,
+    const char* __restrict__ kp, const char* __restrict__ vp) {
+    constexpr int CPR = DP / 4, KT = 1024 / CPR, U = 4, RPW = KT / 4, ST = KT / 16, KS = DP / 16, VN = DP / 64;
+    struct Stage {
+        uint4 k[KT * CPR], v[KT * CPR];
+    };
+    __shared__ __attribute__((aligned(16))) Stage S[2];
+    const PagedCache& c = a.c;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
+    const int G = a.G, D = c.D, page = 1 << c.shift;
+    Seq sq;
+    int b, h, tile;
+    if (!prompt_tile(c, cu, lens, G, 6, &sq, &b, &h, &tile)) return;
+    const int rows = sq.n * G;
+    auto limit = [&](int row) { return limit_of(sq, min(row, rows - 1) / G); };
+    auto uniform = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+    const int w0 = tile * 64 + wave * 16, r = min(w0 + col, rows - 1), qi = r / G, qh = h * G + r - qi * G;
+    const int lim = limit(r), lim_hi = uniform(limit(w0 + 15));
+    const int last = uniform(limit(tile * 64 + 63)), all = uniform(limit(tile * 64));  // positions that any, that every row sees
+    const bool live = w0 < rows;
+
+    const float* qp = static_cast<const float*>(a.q) + (int64_t)(sq.first + qi) * a.q_stride + qh * D;
+    const float sign = a.scale < 0.f ? -1.f : a.scale > 0.f ? 1.f : 0.f;
+    const float cs = fmaxf(fminf(fabsf(a.scale) * 1.44269504088896341f, FLT_MAX), FLT_MIN);
+    floatx4 qf[KS];
+#pragma unroll
+    for (int s = 0; s < KS; s++) {
+        qf[s] = floatx4{0.f, 0.f, 0.f, 0.f};
+        if (16 * s + 4 * g < D) qf[s] = *reinterpret_cast<const floatx4*>(qp + 16 * s + 4 * g);
+        qf[s] *= sign;
+    }
+
+    uint32_t ko[U], vo[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int at = u * 64 + lane, rr = at / CPR, ch = at % CPR, ck = ch ^ ((wave * RPW + rr) & 15);
+        ko[u] = 4 * ck < D ? (uint32_t)(rr * D + 4 * ck) * 4 : 0x7FFFFFF0u;
+        vo[u] = 4 * ch < D ? (uint32_t)(rr * D + 4 * ch) * 4 : 0x7FFFFFF0u;
+    }
+    const int32_t* row = table + (int64_t)b * c.table_stride;
+    const int64_t head = (int64_t)h * page * D;
+    auto page_of = [&](int j0) { return uniform(row[max(min(j0 + wave * RPW, last - 1), 0) >> c.shift]); };
+    auto issue = [&](int j0, int pid, Stage& st) __attribute__((always_inline)) {
+        const int j = j0 + wave * RPW;
+        const bool none = (uint32_t)pid >= (uint32_t)c.n_pages;
+        const int64_t at = ((none ? 0 : pid) * c.page_elems + head + (int64_t)(j & (page - 1)) * D) * 4;
+        const uint32_t bytes = (uint32_t)uniform(none ? 0 : max(min(last - j, RPW), 0) * D * 4);
+        const __amdgpu_buffer_rsrc_t rk = buf_rsrc(kp + at, bytes), rv = buf_rsrc(vp + at, bytes);
+        if (!none) {
+#pragma unroll
+            for (int u = 0; u < U; u++) buf_dma16(rk, ko[u], 0, &st.k[(wave * U + u) * 64]);
+        } else {  // a page that does not exist: NaN scores over zero values
+#pragma unroll
+            for (int u = 0; u < U; u++) st.k[(wave * U + u) * 64 + lane] = make_uint4(0x7FC00000u, 0x7FC00000u, 0x7FC00000u, 0x7FC00000u);
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) buf_dma16(rv, vo[u], 0, &st.v[(wave * U + u) * 64]);
+    };
+
+    float m = -INFINITY, l = 0.f;
+    floatx4 acc[KS];
+#pragma unroll
+    for (int i = 0; i < KS; i++) acc[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+    auto compute = [&](int j0, const char* st, auto edge) __attribute__((always_inline)) {
+        constexpr bool EDGE = decltype(edge)::value;
+        const uint4 *ks = reinterpret_cast<const uint4*>(st), *vs = ks + KT * CPR;
+        floatx4 sc[ST][2];
+#pragma unroll
+        for (int t = 0; t < ST; t++) sc[t][0] = sc[t][1] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < KS; s++)
+#pragma unroll
+            for (int t = 0; t < ST; t++) {
+                const floatx4 kf = __builtin_bit_cast(floatx4, ks[(16 * t + col) * CPR + ((4 * s + g) ^ col)]);
+#pragma unroll
+                for (int e = 0; e < 4; e++) sc[t][e & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[e], qf[s][e], sc[t][e & 1], 0, 0, 0);
+            }
+        float mt = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < ST; t++) {
+            sc[t][0] += sc[t][1];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if (EDGE && j0 + 16 * t + 4 * g + e >= lim) sc[t][0][e] = -INFINITY;
+                mt = fmaxf(mt, sc[t][0][e]);
+            }
+        }
+        mt = lane_pair_max<16>(mt);
+        mt = lane_pair_max<32>(mt);
+        if (__ballot((mt - m) * cs > 8.0f)) {  // (weights stay below 2^8)
+            const float mn = fmaxf(m, mt), al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * cs);
+            m = mn;
+            l *= al;
+#pragma unroll
+            for (int i = 0; i < KS; i++) acc[i] *= al;
+        }
+        const float ms = m == -INFINITY ? 0.f : m;
+        uint32_t wild = 0;
+#pragma unroll
+        for (int t = 0; t < ST; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float p = __builtin_amdgcn_exp2f((sc[t][0][e] - ms) * cs);
+                l += p;
+#pragma unroll
+                for (int i = 0; i < VN; i++) {
+                    uint4 w = vs[(16 * t + 4 * g + e) * CPR + 16 * i + col];
+                    if constexpr (EDGE) {  // infinities and NaN: added below to the rows that see them
+                        uint32_t* u = &w.x;
+#pragma unroll
+                        for (int y = 0; y < 4; y++) {
+                            const uint32_t z = not_finite<float>(u[y]);
+                            wild |= z;
+                            u[y] &= ~z;
+                        }
+                    }
+                    const floatx4 vf = __builtin_bit_cast(floatx4, w);
+#pragma unroll
+                    for (int y = 0; y < 4; y++) acc[4 * i + y] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[y], p, acc[4 * i + y], 0, 0, 0);
+                }
+            }
+        if constexpr (EDGE) {
+            if (__ballot(wild != 0)) {
+#pragma unroll 1
+                for (int k = 0; k < KT && j0 + k < last; k++) {
+                    if (j0 + k >= lim) continue;
+#pragma unroll
+                    for (int i = 0; i < KS; i++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const uint32_t v = reinterpret_cast<const uint32_t*>(vs)[k * DP + 64 * (i / 4) + 4 * (4 * g + e) + i % 4];
+                            acc[i][e] += __uint_as_float(v & not_finite<float>(v));
+                        }
+                }
+            }
+        }
+    };
+
+    const int tiles = (last + KT - 1) / KT, whole = all / KT;
+    if (tiles > 0) {
+        int pid = page_of(0);
+        issue(0, pid, S[0]);
+        pid = page_of(KT);
+        auto step = [&](int t, auto edge) __attribute__((always_inline)) {
+            __builtin_amdgcn_s_waitcnt(0xF70);  // vmcnt(0): this tile's DMA has landed
+            __syncthreads();
+            __builtin_amdgcn_sched_barrier(0);
+            if (t + 1 < tiles) {
+                issue((t + 1) * KT, pid, S[(t + 1) & 1]);
+                pid = page_of((t + 2) * KT);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if (live && t * KT < lim_hi) compute(t * KT, reinterpret_cast<const char*>(&S[t & 1]), edge);
+        };
+        int t = 0;
+#pragma unroll 1
+        for (; t < whole; t++) step(t, std::false_type{});
+#pragma unroll 1
+        for (; t < tiles; t++) step(t, std::true_type{});
+    }
+    l = lane_pair_sum<16>(l);
+    l = lane_pair_sum<32>(l);
+    if (w0 + col >= rows) return;
+    const int sees = sq.shown + qi;
+    const float inv = sees > sq.len ? NAN : 1.0f / l;
+    float* op = static_cast<float*>(a.out) + ((int64_t)(sq.first + qi) * a.hq + qh) * D;
+#pragma unroll
+    for (int i = 0; i < VN; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int d = 64 * i + 4 * (4 * g + e);
+            if (d >= D) continue;
+            floatx4 o = {acc[4 * i][e], acc[4 * i + 1][e], acc[4 * i + 2][e], acc[4 * i + 3][e]};
+            if (sees <= 0) o = floatx4{0.f, 0.f, 0.f, 0.f};
+            else o *= inv;
+            *reinterpret_cast<floatx4*>(op + d) = o;
+        }
+}
+
+// The join, one workgroup per (sequence, KV head, tile) that there can be, in the line's order:
+// for calls whose parts are not joined where they were made.
 template <typename QT>
 __global__ __launch_bounds__(256) void k_paged_join(const PagedAttn a, const int32_t* __restrict__ cu, const int32_t* __restrict__ lens, int keys, int runs) {
-    __shared__ float weight[16][RUNS], total_of[16];
-    __shared__ floatx4 partial[256];
+    __shared__ __attribute__((aligned(16))) float room[JOIN_ROOM];
     const PagedCache& c = a.c;
-    const int G = a.G, D = c.D;
+    const int G = a.G;
     Group grp;
     Seq sq{};
     int64_t total = 0, units = 0, at = -1, nth = 0;
@@ -830,73 +1136,12 @@ __global__ __launch_bounds__(256) void k_paged_join(const PagedAttn a, const int
     }
     if (b < 0) return;
     const Work w = work_of(sq, G, keys);
-    const int64_t len_run = total <= runs ? 1 : (total + runs - 1) / runs;
-    const int64_t x = at + nth * w.rounds;
-    const int64_t run0 = x / len_run, run1 = w.rounds ? (x + w.rounds - 1) / len_run : run0;
-    if (w.rounds && run0 == run1) return;
-    const int h = (int)(nth / w.tiles), tile = (int)(nth - (int64_t)h * w.tiles);
-    const int parts = w.rounds ? (int)(run1 - run0 + 1) : 0, R = min(16, sq.n * G - tile * 16), per = D / 4;
-    const float* rec = a.ws + (2 * run0 + 1) * 16 * (D + 4);  // then slot 0 of run0 + 1, run0 + 2, ...
-    auto part = [&](int i) { return i == 0 ? rec : rec + (2 * i - 1) * (int64_t)(16 * (D + 4)); };
-    // the parts' weights: a wavefront per row, a lane per part
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int r = wave; r < R; r += 4) {
-        float m[RUNS / 64], l[RUNS / 64], cs = 0.f, M = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < RUNS / 64; i++) {
-            m[i] = -INFINITY, l[i] = 0.f;
-            if (64 * i + lane < parts) {
-                const floatx4 z = *reinterpret_cast<const floatx4*>(part(64 * i + lane) + r * (D + 4) + D);
-                m[i] = z[0], l[i] = z[1], cs = z[2];
-            }
-            M = fmaxf(M, m[i]);
-        }
-        M = wave_allmax(M);
-        cs = wave_allmax(cs);  // one value for all parts, at least FLT_MIN
-        const float Ms = M == -INFINITY ? 0.f : M;
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < RUNS / 64; i++)
-            if (64 * i + lane < parts) {
-                const float f = __builtin_amdgcn_exp2f((m[i] - Ms) * cs);
-                sum = fmaf(l[i], f, sum);
-                weight[r][64 * i + lane] = f;
-            }
-        sum = wave_allsum(sum);
-        if (lane == 0) total_of[r] = sum;
-    }
-    __syncthreads();
-    // few rows: the parts in slices, added in order
-    const int items = R * per, slices = max(256 / items, 1);
-    auto put = [&](int it, floatx4 o) {
-        const int r = it / per, dim = 4 * (it - r * per), orow = tile * 16 + r, oq = orow / G, sees = sq.shown + oq;
-        o *= sees > sq.len ? NAN : 1.0f / total_of[r];
-        if (sees <= 0) o = floatx4{0.f, 0.f, 0.f, 0.f};
-        QT* op = static_cast<QT*>(a.out) + ((int64_t)(sq.first + oq) * a.hq + h * G + orow - oq * G) * D;
-        if constexpr (std::is_same_v<QT, float>) *reinterpret_cast<floatx4*>(op + dim) = o;
-        else *reinterpret_cast<half4v*>(op + dim) = half4v{(_Float16)o[0], (_Float16)o[1], (_Float16)o[2], (_Float16)o[3]};
-    };
-    const int slice = slices > 1 ? (int)threadIdx.x / items : 0;
-    for (int it = slices > 1 ? (int)threadIdx.x - slice * items : (int)threadIdx.x; it < items; it += 256) {
-        if (slice >= slices) break;
-        const int r = it / per, at4 = r * (D + 4) + 4 * (it - r * per);
-        floatx4 o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-        for (int i = slice; i < parts; i += slices) {
-            const floatx4 z = *reinterpret_cast<const floatx4*>(part(i) + at4);
-            const float f = weight[r][i];
-#pragma unroll
-            for (int e = 0; e < 4; e++) o[e] = fmaf(z[e], f, o[e]);
-        }
-        if (slices == 1) put(it, o);
-        else partial[threadIdx.x] = o;
-    }
-    if (slices == 1) return;
-    __syncthreads();
-    if ((int)threadIdx.x >= items) return;
-    floatx4 o = partial[threadIdx.x];
-    for (int i = 1; i < slices; i++) o += partial[threadIdx.x + i * items];
-    put(threadIdx.x, o);
+    if (w.rounds == 0) return;
+    const int64_t len_run = run_length(total, runs), x = at + nth * w.rounds;
+    const int run0 = (int)div_u(x, len_run), run1 = (int)div_u(x + w.rounds - 1, len_run);
+    if (run0 == run1) return;
+    const int h = (int)div_u(nth, w.tiles), tile = (int)(nth - (int64_t)h * w.tiles);
+    join_tile<QT, 0>(a, sq, h, tile, run0, run1 - run0 + 1, room);
 }
 
 size_t paged_attention_workspace(int64_t batch, int64_t rows, int hq, int hkv, int D) {
@@ -911,7 +1156,7 @@ static int launch_tile_of(const PagedAttn& a, hipStream_t s) {
     const int64_t most = units * cdiv(a.c.capacity, KEYS);
     const int runs = (int)(most < RUNS ? most : RUNS);
     k_paged_tile<KVT, QT, DP, TK, FULL><<<dim3((unsigned)runs), 256, 0, s>>>(a, a.c.table, a.c.cu, a.c.lens, static_cast<const char*>(a.c.k), static_cast<const char*>(a.c.v));
-    k_paged_join<QT><<<dim3((unsigned)units), 256, 0, s>>>(a, a.c.cu, a.c.lens, KEYS, runs);
+    if (!a.fuse) k_paged_join<QT><<<dim3((unsigned)units), 256, 0, s>>>(a, a.c.cu, a.c.lens, KEYS, runs);
     hipError_t e = hipGetLastError();
     return e == hipSuccess ? TL_HIP_OK : hip_fail(e, "paged attention launch");
 }
@@ -921,10 +1166,14 @@ static int launch_tile(const PagedAttn& a, hipStream_t s) {
     return a.c.D == DP ? launch_tile_of<KVT, QT, DP, TK, true>(a, s) : launch_tile_of<KVT, QT, DP, TK, false>(a, s);
 }
 
-template <typename QT, int DP>
+template <typename KVT, typename QT, int DP>
 static int launch_prompt(const PagedAttn& a, hipStream_t s) {
-    const int64_t units = a.c.hkv * (cdiv((int64_t)a.c.rows * a.G, 128) + a.c.batch);
-    k_paged_prompt<QT, DP><<<dim3((unsigned)units), 256, 0, s>>>(a, a.c.table, a.c.cu, a.c.lens, static_cast<const char*>(a.c.k), static_cast<const char*>(a.c.v));
+    constexpr bool H16 = std::is_same_v<KVT, _Float16>;
+    const int64_t units = a.c.hkv * (cdiv((int64_t)a.c.rows * a.G, H16 ? 128 : 64) + a.c.batch);
+    if constexpr (!H16)
+        k_paged_prompt_f32<DP><<<dim3((unsigned)units), 256, 0, s>>>(a, a.c.table, a.c.cu, a.c.lens, static_cast<const char*>(a.c.k), static_cast<const char*>(a.c.v));
+    else
+        k_paged_prompt<QT, DP><<<dim3((unsigned)units), 256, 0, s>>>(a, a.c.table, a.c.cu, a.c.lens, static_cast<const char*>(a.c.k), static_cast<const char*>(a.c.v));
     hipError_t e = hipGetLastError();
     return e == hipSuccess ? TL_HIP_OK : hip_fail(e, "paged attention launch");
 }
@@ -932,12 +1181,10 @@ static int launch_prompt(const PagedAttn& a, hipStream_t s) {
 template <typename KVT, typename QT>
 static int launch_kind(const PagedAttn& a, hipStream_t s) {
     constexpr bool H16 = std::is_same_v<KVT, _Float16>;
-    if constexpr (H16) {
-        if (a.c.cu && (int64_t)a.c.rows * a.G >= 128 * (int64_t)a.c.batch) {
-            if (a.c.D <= 64) return launch_prompt<QT, 64>(a, s);
-            if (a.c.D <= 128) return launch_prompt<QT, 128>(a, s);
-            return launch_prompt<QT, 256>(a, s);
-        }
+    if (a.c.cu && (int64_t)a.c.rows * a.G >= 128 * (int64_t)a.c.batch) {
+        if (a.c.D <= 64) return launch_prompt<KVT, QT, 64>(a, s);
+        if (a.c.D <= 128) return launch_prompt<KVT, QT, 128>(a, s);
+        return launch_prompt<KVT, QT, 256>(a, s);
     }
     if (a.c.D <= 64) return launch_tile<KVT, QT, 64, 2>(a, s);
     if (a.c.D == 128) return launch_tile_of<KVT, QT, 128, H16 ? 2 : 1, true>(a, s);
