@@ -222,7 +222,7 @@ int tl_hip_debug_last_gemm_plan(int* tile_m, int* tile_n, int* k_splits);
  * The integer arrays are device memory and read by the kernels (a captured call follows their
  * current values at each replay); what they may hold is checked there, never followed out of
  * range: values of cu_seqlens outside 0 .. n_tokens and kv_lens outside 0 .. table_stride *
- * page_size are taken as the nearest bound.  A table entry outside 0 .. n_pages - 1 makes the
+ * page_size are taken as the nearest bound, and a row belongs to the first sequence that claims it.  A table entry outside 0 .. n_pages - 1 makes the
  * attention rows that see its positions NaN, and appends nothing; so does a kv_lens past the
  * table's positions for the rows at positions past them.  Entries past a sequence's length are
  * not read.

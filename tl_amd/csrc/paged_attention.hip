@@ -29,17 +29,29 @@ constexpr int RUNS = 512;  // at most: two workgroups per CU
 struct Seq {
     int first, n, len, shown;
 };
+// Groups are loaded in order from 0: a sequence's rows begin behind those of all before it, so
+// that they never add up to more than the call's, whatever cu holds.
 struct Group {
     Seq q;
-    int base;
+    int base, reach;  // reach: the end of the rows of this group and those before
     __device__ __forceinline__ void load(const PagedCache& c, const int32_t* cu, const int32_t* lens, int from) {
+        const int behind = from == 0 ? 0 : reach;
         base = from;
         const int b = from + (int)__lane_id();
-        q = Seq{0, 0, 0, 0};
-        if (b >= c.batch) return;
-        int n = lens[b], lo = b, hi = b + 1;  // (requested together)
-        if (cu) lo = cu[b], hi = cu[b + 1];
+        int n = 0, lo = 0, hi = 0;
+        if (b < c.batch) {
+            n = lens[b], lo = b, hi = b + 1;  // (requested together)
+            if (cu) lo = cu[b], hi = cu[b + 1];
+        }
         lo = min(max(lo, 0), c.rows), hi = min(max(hi, 0), c.rows), n = min(max(n, 0), INT32_MAX - 32);
+        if (cu) {
+            int top = max(hi, behind);
+#pragma unroll
+            for (int off = 1; off < 64; off <<= 1) top = max(top, __shfl_up(top, off));  // (lanes below off get their own)
+            const int before = __shfl_up(top, 1);
+            lo = max(lo, __lane_id() ? before : behind);
+            reach = __builtin_amdgcn_readlane(top, 63);
+        }
         q.first = lo, q.n = max(hi - lo, 0), q.len = min(n, c.capacity), q.shown = n - q.n + 1;
     }
     __device__ __forceinline__ Seq at(int b) const {
@@ -47,9 +59,9 @@ struct Group {
         return Seq{__builtin_amdgcn_readlane(q.first, i), __builtin_amdgcn_readlane(q.n, i), __builtin_amdgcn_readlane(q.len, i),
                    __builtin_amdgcn_readlane(q.shown, i)};
     }
-    // the same, from another group where b lies there
+    // the same, from a later group where b lies there
     __device__ __forceinline__ Seq at(const PagedCache& c, const int32_t* cu, const int32_t* lens, int b) {
-        if (b - base >= 64) load(c, cu, lens, b & ~63);
+        while (b - base >= 64) load(c, cu, lens, base + 64);
         return at(b);
     }
 };
@@ -92,16 +104,17 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
     return (top - (top >> 15)) | top;
 }
 
-// Adds the parts of a tile that runs run0 .. run0 + parts - 1 left, in order, and writes its rows:
-// a thread per four elements, over all parts or, where the rows are few, over every `slices`-th
+// Adds the parts of a tile's records, in order, and writes its rows: part 0 at byte `first` of the
+// workspace, part i at rest + i step.  A thread per four elements, over all parts or, where the rows are few, over every `slices`-th
 // and then over the slices.  Eight parts are requested at a time.
 constexpr int JOIN_ROOM = 256 * 7;  // floats of LDS
 template <typename QT, int POLICY>
-__device__ __forceinline__ void join_tile(const PagedAttn& a, const Seq& sq, int h, int tile, int run0, int parts, float* room) {
+__device__ __forceinline__ void join_tile(const PagedAttn& a, const Seq& sq, int h, int tile, uint32_t first, uint32_t rest,
+                                          uint32_t step, int parts, uint32_t bytes, float* room) {
     const int G = a.G, D = a.c.D, R = min(16, sq.n * G - tile * 16), per = D / 4;
-    const uint32_t rec = 16 * (D + 4) * 4, row = (D + 4) * 4;  // bytes
-    const __amdgpu_buffer_rsrc_t ws = buf_rsrc(a.ws, RUNS * 2 * rec);
-    auto part = [&](int i) { return (uint32_t)(2 * (run0 + i) + (i == 0 ? 1 : 0)) * rec; };  // the first in slot 1, the rest in slot 0
+    const uint32_t row = (D + 4) * 4;
+    const __amdgpu_buffer_rsrc_t ws = buf_rsrc(a.ws, bytes);
+    auto part = [&](int i) { return i == 0 ? first : rest + (uint32_t)i * step; };
     auto word4 = [&](uint32_t at) { return __builtin_bit_cast(floatx4, __builtin_amdgcn_raw_buffer_load_b128(ws, at, 0, POLICY)); };
     floatx4* po = reinterpret_cast<floatx4*>(room);
     float *pm = room + 1024, *pl = room + 1280;
@@ -135,7 +148,7 @@ __device__ __forceinline__ void join_tile(const PagedAttn& a, const Seq& sq, int
 #pragma unroll
             for (int u = 0; u < 8; u++) {
                 // (an offset at the resource's end reads nothing)
-                const uint32_t at = i0 + u * slices < parts ? part(i0 + u * slices) + r * row : RUNS * 2 * rec;
+                const uint32_t at = i0 + u * slices < parts ? part(i0 + u * slices) + r * row : bytes;
                 z[u] = word4(at + 16 * (it - r * per));
                 ml[u] = word4(at + 4 * D);
             }
@@ -161,6 +174,12 @@ __device__ __forceinline__ void join_tile(const PagedAttn& a, const Seq& sq, int
     for (int i = 1; i < slices; i++)
         if (i < parts) add(t, po[it + i * items], pm[it + i * items], pl[it + i * items]);
     put(it, t);
+}
+// Runs run0 .. run0 + parts - 1 of k_paged_tile: the first run's record in its slot 1, the others' in slot 0.
+template <typename QT, int POLICY>
+__device__ __forceinline__ void join_run(const PagedAttn& a, const Seq& sq, int h, int tile, int run0, int parts, float* room) {
+    const uint32_t rec = 16 * (a.c.D + 4) * 4;
+    join_tile<QT, POLICY>(a, sq, h, tile, (2 * run0 + 1) * rec, 2 * run0 * rec, 2 * rec, parts, RUNS * 2 * rec, room);
 }
 // One launch: arrivals at the tile that run `i` began, zero between calls.  The run that arrives
 // last joins the tile and sets its counter back.
@@ -620,18 +639,26 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_tile(
                 last_here = end;
             }
             __syncthreads();
-            if (last_here) join_tile<QT, CPOL_SC1>(a, sq, h, tile, run0, parts, &so[0][0][0]);
+            if (last_here) join_run<QT, CPOL_SC1>(a, sq, h, tile, run0, parts, &so[0][0][0]);
         }
     }
 }
 
-// The tile of 2^shift rows that a workgroup of the prompt kernels takes: KV heads next to each
-// other (on XCDs of their own), tiles from the last one back, so that of one sequence the longest
-// come first.
-__device__ __forceinline__ bool prompt_tile(const PagedCache& c, const int32_t* cu, const int32_t* lens, int G, int shift, Seq* sq,
-                                            int* b, int* h, int* tile) {
-    *h = blockIdx.x % c.hkv;
-    const int back = blockIdx.x / c.hkv, up = (1 << shift) - 1;
+// ---- prompts: which work is whose ----
+// Tiles of 2^shift rows, `unit` = KV head + n_kv_heads * tile: heads next to each other (on XCDs
+// of their own), tiles from the last one back, so that of one sequence the longest come first.
+// A call with few units cuts each unit's positions into SLOTS / units parts, of about four K/V
+// tiles at least; a workgroup takes unit blockIdx % units, part blockIdx / units, and leaves a
+// record (o, m, l, c of its rows) in slot unit * (SLOTS / units) + part, which k_prompt_join adds.
+constexpr int SLOTS = 512;
+struct Prompt {
+    Seq sq;
+    int b, h, tile, unit, units, most;  // most: parts per unit, at most
+};
+// cut: whether units are cut; index: the workgroup's, or with cut the one of SLOTS.
+__device__ __forceinline__ bool prompt_tile(const PagedCache& c, const int32_t* cu, const int32_t* lens, int G, int shift, int index,
+                                            bool cut, bool whole_units, Prompt* p) {
+    const int up = (1 << shift) - 1;
     Group grp;
     int64_t total = 0, incl = 0, mine = 0;
     for (int base = 0; base < c.batch; base += 64) {
@@ -640,8 +667,13 @@ __device__ __forceinline__ bool prompt_tile(const PagedCache& c, const int32_t* 
         incl = lane_prefix(mine);
         total += lane_value(incl, 63);
     }
-    const int64_t nth = total - 1 - back;
-    if (nth < 0) return false;
+    p->units = (int)(total * c.hkv);  // (rows and heads together are below 2^27)
+    if (p->units == 0) return false;
+    p->most = cut ? max(SLOTS / p->units, 1) : 1;
+    p->unit = cut && !whole_units ? index % p->units : index;
+    if (p->unit >= p->units) return false;
+    p->h = p->unit % c.hkv;
+    const int64_t nth = total - 1 - p->unit / c.hkv;
     int64_t before = 0;
     for (int base = 0;; base += 64) {
         if (c.batch > 64) {
@@ -652,15 +684,17 @@ __device__ __forceinline__ bool prompt_tile(const PagedCache& c, const int32_t* 
         const uint64_t hit = __ballot(nth < before + incl);
         if (hit) {
             const int at = __builtin_ctzll(hit);
-            *b = base + at;
-            *tile = __builtin_amdgcn_readfirstlane((int)(nth - (before + lane_value(incl, at) - lane_value(mine, at))));
+            p->b = base + at;
+            p->tile = __builtin_amdgcn_readfirstlane((int)(nth - (before + lane_value(incl, at) - lane_value(mine, at))));
             break;
         }
         before += lane_value(incl, 63);
     }
-    *sq = grp.at(*b);
+    p->sq = grp.at(p->b);
     return true;
 }
+// Parts of a unit with this many K/V tiles.
+__device__ __forceinline__ int prompt_parts(int most, int tiles) { return max(min(most, (tiles + 3) / 4), 1); }
 
 // ---- prompts over f16 caches -------------------------------------------------------------
 // A workgroup takes 128 rows, a wavefront 32 of them; 64 positions (32 at head sizes past 128) at
@@ -687,7 +721,7 @@ typedef short short4v __attribute__((ext_vector_type(4)));
 template <typename QT, int DP>
 __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_prompt(
     const PagedAttn a, const int32_t* __restrict__ table, const int32_t* __restrict__ cu, const int32_t* __restrict__ lens,
-    const char* __restrict__ kp, const char* __restrict__ vp) {
+    const char* __restrict__ kp, const char* __restrict__ vp, bool cut) {
     using L = PromptTile<DP>;
     constexpr int KT = L::KT, CPR = L::CPR, U = L::U, RPW = KT / 4;
     constexpr int QP = std::is_same_v<QT, float> ? 2 : 1;  // f16 parts of a query, and of a weight
@@ -700,9 +734,10 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_prompt(
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, hf = lane >> 5;
     const int G = a.G, D = c.D, page = 1 << c.shift;
 
-    Seq sq;
-    int b, h, tile;
-    if (!prompt_tile(c, cu, lens, G, 7, &sq, &b, &h, &tile)) return;
+    Prompt pt;
+    if (!prompt_tile(c, cu, lens, G, 7, blockIdx.x, cut, false, &pt)) return;
+    const Seq sq = pt.sq;
+    const int b = pt.b, h = pt.h, tile = pt.tile;
     const int rows = sq.n * G;
     auto limit = [&](int row) { return limit_of(sq, min(row, rows - 1) / G); };
     auto uniform = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
@@ -710,6 +745,10 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_prompt(
     const int lim = limit(r), lim_hi = uniform(limit(w0 + 31));
     const int last = uniform(limit(tile * 128 + 127)), all = uniform(limit(tile * 128));  // positions that any, that every row sees
     const bool live = w0 < rows;
+    // this part's K/V tiles
+    const int tiles = (last + KT - 1) / KT, whole = all / KT, parts = prompt_parts(pt.most, tiles), part = blockIdx.x / pt.units;
+    if (cut && part >= parts) return;
+    const int t0 = cut ? (int)((int64_t)tiles * part / parts) : 0, t1 = cut ? (int)((int64_t)tiles * (part + 1) / parts) : tiles;
 
     // this lane's part of its row: dimensions 16 s + 8 hf ..
     const QT* qp = static_cast<const QT*>(a.q) + (int64_t)(sq.first + qi) * a.q_stride + qh * D;
@@ -881,33 +920,34 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_prompt(
         }
     };
 
-    const int tiles = (last + KT - 1) / KT, whole = all / KT;
-    if (tiles > 0) {
-        int pid = page_of(0);
-        issue(0, pid, S[0]);
-        pid = page_of(KT);
+    if (t0 < t1) {
+        int pid = page_of(t0 * KT);
+        issue(t0 * KT, pid, S[t0 & 1]);
+        pid = page_of((t0 + 1) * KT);
         auto step = [&](int t, auto edge) __attribute__((always_inline)) {
             __builtin_amdgcn_s_waitcnt(0xF70);  // vmcnt(0): this tile's DMA has landed
             __syncthreads();
             __builtin_amdgcn_sched_barrier(0);
-            if (t + 1 < tiles) {
+            if (t + 1 < t1) {
                 issue((t + 1) * KT, pid, S[(t + 1) & 1]);
                 pid = page_of((t + 2) * KT);
             }
             __builtin_amdgcn_sched_barrier(0);
             if (live && t * KT < lim_hi) compute(t * KT, reinterpret_cast<const char*>(&S[t & 1]), edge);
         };
-        int t = 0;
+        int t = t0;
 #pragma unroll 1
-        for (; t < whole; t++) step(t, std::false_type{});
+        for (; t < min(whole, t1); t++) step(t, std::false_type{});
 #pragma unroll 1
-        for (; t < tiles; t++) step(t, std::true_type{});
+        for (; t < t1; t++) step(t, std::true_type{});
     }
     l = lane_pair_sum<32>(l);
     if (w0 + col >= rows) return;
     const int sees = sq.shown + qi;
     const float inv = sees > sq.len ? NAN : 1.0f / l;
     QT* op = static_cast<QT*>(a.out) + ((int64_t)(sq.first + qi) * a.hq + qh) * D;
+    float* rec = a.ws + ((int64_t)(pt.unit * pt.most + part) * 128 + wave * 32 + col) * (D + 4);
+    if (parts > 1 && hf == 0) *reinterpret_cast<floatx4*>(rec + D) = floatx4{m, l, cs, 0.f};
 #pragma unroll
     for (int i = 0; i < DT; i++)
 #pragma unroll
@@ -915,6 +955,10 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_prompt(
             const int d = 32 * i + 8 * e + 4 * hf;
             if (d >= D) continue;
             floatx4 o = {acc[i][4 * e], acc[i][4 * e + 1], acc[i][4 * e + 2], acc[i][4 * e + 3]};
+            if (parts > 1) {
+                *reinterpret_cast<floatx4*>(rec + d) = o;
+                continue;
+            }
             if (sees <= 0) o = floatx4{0.f, 0.f, 0.f, 0.f};
             else o *= inv;
             if constexpr (std::is_same_v<QT, float>) *reinterpret_cast<floatx4*>(op + d) = o;
@@ -930,7 +974,7 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_prompt(
 template <int DP>
 __global__ __launch_bounds__(256, 2) void k_paged_prompt_f32(
     const PagedAttn a, const int32_t* __restrict__ table, const int32_t* __restrict__ cu, const int32_t* __restrict__ lens,
-    const char* __restrict__ kp, const char* __restrict__ vp) {
+    const char* __restrict__ kp, const char* __restrict__ vp, bool cut) {
     constexpr int CPR = DP / 4, KT = 1024 / CPR, U = 4, RPW = KT / 4, ST = KT / 16, KS = DP / 16, VN = DP / 64;
     struct Stage {
         uint4 k[KT * CPR], v[KT * CPR];
@@ -939,9 +983,10 @@ __global__ __launch_bounds__(256, 2) void k_paged_prompt_f32(
     const PagedCache& c = a.c;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
     const int G = a.G, D = c.D, page = 1 << c.shift;
-    Seq sq;
-    int b, h, tile;
-    if (!prompt_tile(c, cu, lens, G, 6, &sq, &b, &h, &tile)) return;
+    Prompt pt;
+    if (!prompt_tile(c, cu, lens, G, 6, blockIdx.x, cut, false, &pt)) return;
+    const Seq sq = pt.sq;
+    const int b = pt.b, h = pt.h, tile = pt.tile;
     const int rows = sq.n * G;
     auto limit = [&](int row) { return limit_of(sq, min(row, rows - 1) / G); };
     auto uniform = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
@@ -949,6 +994,10 @@ __global__ __launch_bounds__(256, 2) void k_paged_prompt_f32(
     const int lim = limit(r), lim_hi = uniform(limit(w0 + 15));
     const int last = uniform(limit(tile * 64 + 63)), all = uniform(limit(tile * 64));  // positions that any, that every row sees
     const bool live = w0 < rows;
+    // this part's K/V tiles
+    const int tiles = (last + KT - 1) / KT, whole = all / KT, parts = prompt_parts(pt.most, tiles), part = blockIdx.x / pt.units;
+    if (cut && part >= parts) return;
+    const int t0 = cut ? (int)((int64_t)tiles * part / parts) : 0, t1 = cut ? (int)((int64_t)tiles * (part + 1) / parts) : tiles;
 
     const float* qp = static_cast<const float*>(a.q) + (int64_t)(sq.first + qi) * a.q_stride + qh * D;
     const float sign = a.scale < 0.f ? -1.f : a.scale > 0.f ? 1.f : 0.f;
@@ -1067,27 +1116,26 @@ __global__ __launch_bounds__(256, 2) void k_paged_prompt_f32(
         }
     };
 
-    const int tiles = (last + KT - 1) / KT, whole = all / KT;
-    if (tiles > 0) {
-        int pid = page_of(0);
-        issue(0, pid, S[0]);
-        pid = page_of(KT);
+    if (t0 < t1) {
+        int pid = page_of(t0 * KT);
+        issue(t0 * KT, pid, S[t0 & 1]);
+        pid = page_of((t0 + 1) * KT);
         auto step = [&](int t, auto edge) __attribute__((always_inline)) {
             __builtin_amdgcn_s_waitcnt(0xF70);  // vmcnt(0): this tile's DMA has landed
             __syncthreads();
             __builtin_amdgcn_sched_barrier(0);
-            if (t + 1 < tiles) {
+            if (t + 1 < t1) {
                 issue((t + 1) * KT, pid, S[(t + 1) & 1]);
                 pid = page_of((t + 2) * KT);
             }
             __builtin_amdgcn_sched_barrier(0);
             if (live && t * KT < lim_hi) compute(t * KT, reinterpret_cast<const char*>(&S[t & 1]), edge);
         };
-        int t = 0;
+        int t = t0;
 #pragma unroll 1
-        for (; t < whole; t++) step(t, std::false_type{});
+        for (; t < min(whole, t1); t++) step(t, std::false_type{});
 #pragma unroll 1
-        for (; t < tiles; t++) step(t, std::true_type{});
+        for (; t < t1; t++) step(t, std::true_type{});
     }
     l = lane_pair_sum<16>(l);
     l = lane_pair_sum<32>(l);
@@ -1095,6 +1143,8 @@ __global__ __launch_bounds__(256, 2) void k_paged_prompt_f32(
     const int sees = sq.shown + qi;
     const float inv = sees > sq.len ? NAN : 1.0f / l;
     float* op = static_cast<float*>(a.out) + ((int64_t)(sq.first + qi) * a.hq + qh) * D;
+    float* rec = a.ws + ((int64_t)(pt.unit * pt.most + part) * 64 + wave * 16 + col) * (D + 4);
+    if (parts > 1 && g == 0) *reinterpret_cast<floatx4*>(rec + D) = floatx4{m, l, cs, 0.f};
 #pragma unroll
     for (int i = 0; i < VN; i++)
 #pragma unroll
@@ -1102,10 +1152,31 @@ __global__ __launch_bounds__(256, 2) void k_paged_prompt_f32(
             const int d = 64 * i + 4 * (4 * g + e);
             if (d >= D) continue;
             floatx4 o = {acc[4 * i][e], acc[4 * i + 1][e], acc[4 * i + 2][e], acc[4 * i + 3][e]};
+            if (parts > 1) {
+                *reinterpret_cast<floatx4*>(rec + d) = o;
+                continue;
+            }
             if (sees <= 0) o = floatx4{0.f, 0.f, 0.f, 0.f};
             else o *= inv;
             *reinterpret_cast<floatx4*>(op + d) = o;
         }
+}
+
+// Adds the parts of cut units, 16 rows to a workgroup.
+template <typename QT>
+__global__ __launch_bounds__(256) void k_prompt_join(const PagedAttn a, const int32_t* __restrict__ cu, const int32_t* __restrict__ lens, int shift, int keys) {
+    __shared__ __attribute__((aligned(16))) float room[JOIN_ROOM];
+    const PagedCache& c = a.c;
+    const int G = a.G, per = 1 << (shift - 4), sub = blockIdx.x & (per - 1);
+    Prompt pt;
+    if (!prompt_tile(c, cu, lens, G, shift, blockIdx.x / per, true, true, &pt)) return;
+    const int rows = pt.sq.n * G, r0 = (pt.tile << shift) + 16 * sub;
+    if (r0 >= rows) return;
+    const int last = limit_of(pt.sq, min((pt.tile << shift) + (1 << shift) - 1, rows - 1) / G);
+    const int parts = prompt_parts(pt.most, (last + keys - 1) / keys);
+    if (parts == 1) return;
+    const uint32_t row = (c.D + 4) * 4, slot = row << shift, first = (uint32_t)(pt.unit * pt.most) * slot + 16 * sub * row;
+    join_tile<QT, 0>(a, pt.sq, pt.h, r0 >> 4, first, first, slot, parts, (uint32_t)SLOTS * slot, room);
 }
 
 // The join, one workgroup per (sequence, KV head, tile) that there can be, in the line's order:
@@ -1141,18 +1212,42 @@ __global__ __launch_bounds__(256) void k_paged_join(const PagedAttn a, const int
     const int run0 = (int)div_u(x, len_run), run1 = (int)div_u(x + w.rounds - 1, len_run);
     if (run0 == run1) return;
     const int h = (int)div_u(nth, w.tiles), tile = (int)(nth - (int64_t)h * w.tiles);
-    join_tile<QT, 0>(a, sq, h, tile, run0, run1 - run0 + 1, room);
+    join_run<QT, 0>(a, sq, h, tile, run0, run1 - run0 + 1, room);
 }
 
+// Units that there can be, for tiles of `tile` rows.
+static int64_t units_of(int64_t batch, int64_t rows, int G, int hkv, int tile) { return hkv * (cdiv(rows * G, tile) + batch); }
+// Whether a packed call takes the prompt kernels, which read each K/V row an eighth as often as
+// 16-row tiles, and need a second launch where their units are cut: with many 16-row tiles, or as
+// many rounds of 128 positions in them as the table has room for.  us, 16-row tiles against these,
+// f32 rows, 32 heads over 8 of 128, f16 caches: 8 x 128 rows over nothing (1088 tiles) 31 against
+// 17; 256 rows (520) over nothing 12 against 20, over 2000 48 against 45, over 16000 372 against
+// 146; 8 x 32 rows over 1000 (576) 31 against 35, 8 x 64 (1088) 62 against 43.  f32 caches, 32 over
+// 4 of 64: 8 x 16 rows over 1000 (288) 24 against 22, 256 rows over nothing (516) 13 against 19.
+static bool takes_prompt(int64_t batch, int64_t rows, int G, int hkv, int64_t capacity, bool kv16) {
+    const int64_t tiles = units_of(batch, rows, G, hkv, 16);
+    return tiles >= 1024 || tiles * cdiv(capacity, 128) >= (kv16 ? 8192 : 2048);
+}
+// Whether their units are cut: where they alone, about half a tile per sequence short of the most
+// there can be, would leave CUs idle (256 rows over 16000, 64 units: 447 us whole, 146 cut;
+// 8 x 128 rows over nothing, 256 units: 17 whole, 22 cut).
+static bool cuts(int64_t batch, int64_t rows, int G, int hkv, int tile) { return hkv * (cdiv(rows * G, tile) + batch / 2) < 256; }
+
+// The records of the runs, or of cut prompts where the packed rows may be such, whatever the table.
 size_t paged_attention_workspace(int64_t batch, int64_t rows, int hq, int hkv, int D) {
-    return (size_t)RUNS * 2 * 16 * (D + 4) * sizeof(float);
+    const int G = hq / hkv;
+    size_t most = RUNS * 2 * 16;
+    if (rows > batch)
+        for (const int tile : {64, 128})
+            if (cuts(batch, rows, G, hkv, tile)) most = (size_t)SLOTS * tile;
+    return most * (D + 4) * sizeof(float);
 }
 
 template <typename KVT, typename QT, int DP, int TK, bool FULL>
 static int launch_tile_of(const PagedAttn& a, hipStream_t s) {
     constexpr int KEYS = Tile<KVT, QT, DP, TK>::KEYS;
     // as many runs as there can be rounds, up to two workgroups per CU
-    const int64_t units = a.c.hkv * (a.c.cu ? cdiv((int64_t)a.c.rows * a.G, 16) + a.c.batch : (int64_t)a.c.batch * cdiv(a.G, 16));
+    const int64_t units = a.c.cu ? units_of(a.c.batch, a.c.rows, a.G, a.c.hkv, 16) : (int64_t)a.c.hkv * a.c.batch * cdiv(a.G, 16);
     const int64_t most = units * cdiv(a.c.capacity, KEYS);
     const int runs = (int)(most < RUNS ? most : RUNS);
     k_paged_tile<KVT, QT, DP, TK, FULL><<<dim3((unsigned)runs), 256, 0, s>>>(a, a.c.table, a.c.cu, a.c.lens, static_cast<const char*>(a.c.k), static_cast<const char*>(a.c.v));
@@ -1169,11 +1264,14 @@ static int launch_tile(const PagedAttn& a, hipStream_t s) {
 template <typename KVT, typename QT, int DP>
 static int launch_prompt(const PagedAttn& a, hipStream_t s) {
     constexpr bool H16 = std::is_same_v<KVT, _Float16>;
-    const int64_t units = a.c.hkv * (cdiv((int64_t)a.c.rows * a.G, H16 ? 128 : 64) + a.c.batch);
-    if constexpr (!H16)
-        k_paged_prompt_f32<DP><<<dim3((unsigned)units), 256, 0, s>>>(a, a.c.table, a.c.cu, a.c.lens, static_cast<const char*>(a.c.k), static_cast<const char*>(a.c.v));
-    else
-        k_paged_prompt<QT, DP><<<dim3((unsigned)units), 256, 0, s>>>(a, a.c.table, a.c.cu, a.c.lens, static_cast<const char*>(a.c.k), static_cast<const char*>(a.c.v));
+    constexpr int ROWS = H16 ? 128 : 64, KEYS = H16 ? PromptTile<DP>::KT : 4096 / DP;
+    const int64_t units = units_of(a.c.batch, a.c.rows, a.G, a.c.hkv, ROWS);
+    const bool cut = cuts(a.c.batch, a.c.rows, a.G, a.c.hkv, ROWS);
+    const dim3 grid((unsigned)(cut ? SLOTS : units));
+    const char *kp = static_cast<const char*>(a.c.k), *vp = static_cast<const char*>(a.c.v);
+    if constexpr (H16) k_paged_prompt<QT, DP><<<grid, 256, 0, s>>>(a, a.c.table, a.c.cu, a.c.lens, kp, vp, cut);
+    else k_paged_prompt_f32<DP><<<grid, 256, 0, s>>>(a, a.c.table, a.c.cu, a.c.lens, kp, vp, cut);
+    if (cut) k_prompt_join<QT><<<dim3((unsigned)(units * (ROWS / 16))), 256, 0, s>>>(a, a.c.cu, a.c.lens, H16 ? 7 : 6, KEYS);
     hipError_t e = hipGetLastError();
     return e == hipSuccess ? TL_HIP_OK : hip_fail(e, "paged attention launch");
 }
@@ -1181,7 +1279,7 @@ static int launch_prompt(const PagedAttn& a, hipStream_t s) {
 template <typename KVT, typename QT>
 static int launch_kind(const PagedAttn& a, hipStream_t s) {
     constexpr bool H16 = std::is_same_v<KVT, _Float16>;
-    if (a.c.cu && (int64_t)a.c.rows * a.G >= 128 * (int64_t)a.c.batch) {
+    if (a.c.cu && a.c.rows > a.c.batch && takes_prompt(a.c.batch, a.c.rows, a.G, a.c.hkv, a.c.capacity, H16)) {
         if (a.c.D <= 64) return launch_prompt<KVT, QT, 64>(a, s);
         if (a.c.D <= 128) return launch_prompt<KVT, QT, 128>(a, s);
         return launch_prompt<KVT, QT, 256>(a, s);
