@@ -17,22 +17,51 @@ struct PagedCache {
     int32_t capacity;              // table_stride * page
 };
 
-// Positions of sequence b that the table can hold, and whether kv_lens asks for more.
-__device__ __forceinline__ int paged_len(const PagedCache& c, int b, bool* past) {
-    const int n = c.lens[b];
-    *past = n > c.capacity;
-    return min(max(n, 0), c.capacity);
-}
-// First packed row of sequence b and the number of its rows.
-__device__ __forceinline__ int paged_rows(const PagedCache& c, int b, int* first) {
-    if (!c.cu) {
-        *first = b;
-        return 1;
+// Sequences base + lane: packed rows first .. first + n - 1, positions len that the table holds,
+// and `shown` positions that its row 0 sees (0 or fewer: none).
+struct Seq {
+    int first, n, len, shown;
+};
+// Groups are loaded in order from 0: a sequence's rows begin behind those of all before it, so
+// that they never add up to more than the call's, whatever cu holds.
+template <bool PACKED>  // otherwise one row per sequence
+struct Group {
+    Seq q;
+    int base, reach;  // reach: the end of the rows of this group and those before
+    __device__ __forceinline__ void load(const PagedCache& c, const int32_t* cu, const int32_t* lens, int from) {
+        [[maybe_unused]] const int behind = from == 0 ? 0 : reach;
+        base = from;
+        const int b = from + (int)__lane_id();
+        int n = 0, lo = 0, hi = 0;
+        if (b < c.batch) {
+            n = lens[b], lo = b, hi = b + 1;  // (requested together)
+            if constexpr (PACKED) lo = cu[b], hi = cu[b + 1];
+        }
+        n = min(max(n, 0), INT32_MAX - 32);
+        if constexpr (PACKED) {
+            lo = min(max(lo, 0), c.rows), hi = min(max(hi, 0), c.rows);
+            int top = max(hi, behind);
+#pragma unroll
+            for (int off = 1; off < 64; off <<= 1) top = max(top, __shfl_up(top, off));  // (lanes below off get their own)
+            const int before = __shfl_up(top, 1);
+            lo = max(lo, __lane_id() ? before : behind);
+            reach = __builtin_amdgcn_readlane(top, 63);
+        }
+        q.first = lo, q.n = max(hi - lo, 0), q.len = min(n, c.capacity), q.shown = n - q.n + 1;
     }
-    const int lo = min(max(c.cu[b], 0), c.rows), hi = min(max(c.cu[b + 1], 0), c.rows);
-    *first = lo;
-    return max(hi - lo, 0);
-}
+    __device__ __forceinline__ Seq at(int b) const {
+        const int i = b - base;
+        return Seq{__builtin_amdgcn_readlane(q.first, i), __builtin_amdgcn_readlane(q.n, i), __builtin_amdgcn_readlane(q.len, i),
+                   __builtin_amdgcn_readlane(q.shown, i)};
+    }
+    // the same, from a later group where b lies there
+    __device__ __forceinline__ Seq at(const PagedCache& c, const int32_t* cu, const int32_t* lens, int b) {
+        while (b - base >= 64) load(c, cu, lens, base + 64);
+        return at(b);
+    }
+};
+// Positions that row i of a sequence sees.
+__device__ __forceinline__ int limit_of(const Seq& q, int i) { return max(min(q.shown + i, q.len), 0); }
 
 struct PagedAttn {
     PagedCache c;

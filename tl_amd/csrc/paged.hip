@@ -12,6 +12,10 @@
 namespace tlhip {
 
 // ---- append --------------------------------------------------------------------------
+// Every new row is read once and written once: HBM bound.  A workgroup takes TOKENS rows, a thread
+// the same 8 elements of each (16-byte stores, the loads of all rows requested first); its
+// wavefronts find the rows' places for themselves, a lane per sequence.  8192 f32 rows of 8 heads of
+// 128 into f16 pages (101 MB): 20.8 us, 4.8 TB/s, with 1 to 4 rows per workgroup alike.
 struct AppendArgs {
     PagedCache c;
     const void* kn;
@@ -19,36 +23,58 @@ struct AppendArgs {
     int64_t ks, vs;  // row strides in elements
 };
 
-template <typename NT, typename KVT>
-__global__ __launch_bounds__(256) void k_kv_append(const AppendArgs a) {
+template <typename NT, typename KVT, int TOKENS>
+__global__ __launch_bounds__(256) void k_kv_append(const AppendArgs a, const int32_t* __restrict__ table, const int32_t* __restrict__ cu,
+                                                   const int32_t* __restrict__ lens) {
     const PagedCache& c = a.c;
-    const int per = c.hkv * (c.D >> 3);  // 8-element chunks of a row
-    const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t t64 = u / (2 * per);
-    if (t64 >= c.rows) return;
-    const int t = (int)t64, r = (int)(u - t64 * 2 * per), isv = r >= per, ch = isv ? r - per : r;
-    int b = 0, first = 0, n = 0;
-    for (; b < c.batch; b++) {
-        n = paged_rows(c, b, &first);
-        if (t >= first && t < first + n) break;
-    }
-    if (b == c.batch) return;
-    const int64_t j = (int64_t)c.lens[b] - n + (t - first);
-    if (j < 0 || j >= c.capacity) return;
-    const int p = c.table[b * c.table_stride + (j >> c.shift)];
-    if ((uint32_t)p >= (uint32_t)c.n_pages) return;
-    const int h = ch / (c.D >> 3), d = (ch - h * (c.D >> 3)) * 8, page = 1 << c.shift;
-    const NT* src = isv ? static_cast<const NT*>(a.vn) + t * a.vs : static_cast<const NT*>(a.kn) + t * a.ks;
-    KVT* dst = static_cast<KVT*>(const_cast<void*>(isv ? c.v : c.k)) + p * c.page_elems + ((int64_t)h * page + (j & (page - 1))) * c.D;
+    const int t0 = blockIdx.x * TOKENS, page = 1 << c.shift;
+    // where each row goes, in elements from the pool's start: -1 nowhere
+    int64_t to[TOKENS];
 #pragma unroll
-    for (int i = 0; i < 8; i++) dst[d + i] = (KVT)(float)src[h * c.D + d + i];
+    for (int i = 0; i < TOKENS; i++) to[i] = -1;
+    Group<true> grp;
+    for (int base = 0; base < c.batch; base += 64) {
+        grp.load(c, cu, lens, base);
+#pragma unroll
+        for (int i = 0; i < TOKENS; i++) {
+            const uint64_t hit = __ballot(t0 + i >= grp.q.first && t0 + i < grp.q.first + grp.q.n);
+            if (!hit) continue;
+            const int b = base + __builtin_ctzll(hit);
+            const Seq s = grp.at(b);
+            const int j = s.shown - 1 + (t0 + i - s.first);  // its position
+            if (j < 0 || j >= c.capacity) continue;
+            const int p = table[(int64_t)b * c.table_stride + (j >> c.shift)];
+            if ((uint32_t)p < (uint32_t)c.n_pages) to[i] = p * c.page_elems + (int64_t)(j & (page - 1)) * c.D;
+        }
+    }
+    const int per = c.D >> 3, row = c.hkv * per;  // chunks of 8 elements
+    typedef NT in8 __attribute__((ext_vector_type(8)));
+    typedef KVT out8 __attribute__((ext_vector_type(8)));
+    for (int u = threadIdx.x; u < 2 * row; u += 256) {
+        const bool isv = u >= row;
+        const int ch = isv ? u - row : u, h = ch / per;
+        const NT* src = (isv ? static_cast<const NT*>(a.vn) + t0 * a.vs : static_cast<const NT*>(a.kn) + t0 * a.ks) + 8 * ch;
+        KVT* dst = static_cast<KVT*>(const_cast<void*>(isv ? c.v : c.k)) + (int64_t)h * page * c.D + 8 * (ch - h * per);
+        const int64_t step = isv ? a.vs : a.ks;
+        in8 x[TOKENS];
+#pragma unroll
+        for (int i = 0; i < TOKENS; i++)
+            if (to[i] >= 0) x[i] = *reinterpret_cast<const in8*>(src + i * step);
+#pragma unroll
+        for (int i = 0; i < TOKENS; i++)
+            if (to[i] >= 0) *reinterpret_cast<out8*>(dst + to[i]) = __builtin_convertvector(x[i], out8);
+    }
 }
 
 // ---- page copies ---------------------------------------------------------------------
-constexpr int COPY_PAIRS = 440;  // in the kernel's arguments (at most 4 KiB): nothing to upload
+// Bytes read and written once: HBM bound.  The pairs travel in the kernel's arguments (at most
+// 4 KiB): nothing to upload, and a captured call keeps its own.  16 bytes per thread, past the
+// caches: 768 pages of 128 KiB, K and V (403 MB) 68.8 us, 5.9 TB/s (74.9 us through the caches;
+// 79.8 with four loads per thread).
+constexpr int COPY_PAIRS = 440;
 struct CopyArgs {
-    uint4* k;
-    uint4* v;
+    u32x4* k;
+    u32x4* v;
     int64_t layer;  // 16-byte words of a layer, and of a page
     int64_t page;
     int32_t src[COPY_PAIRS], dst[COPY_PAIRS];
@@ -57,8 +83,8 @@ struct CopyArgs {
 __global__ __launch_bounds__(256) void k_kv_copy(const CopyArgs a) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= a.page) return;
-    uint4* p = (blockIdx.z & 1 ? a.v : a.k) + (blockIdx.z >> 1) * a.layer;
-    p[a.dst[blockIdx.y] * a.page + i] = p[a.src[blockIdx.y] * a.page + i];
+    u32x4* p = (blockIdx.z & 1 ? a.v : a.k) + (blockIdx.z >> 1) * a.layer + i;
+    __builtin_nontemporal_store(__builtin_nontemporal_load(p + a.src[blockIdx.y] * a.page), p + a.dst[blockIdx.y] * a.page);
 }
 
 // ---- checks --------------------------------------------------------------------------
@@ -99,7 +125,6 @@ static int check_heads(int hq, int hkv) {
 struct OnStream {
     hipStream_t s = nullptr;
     int rc = TL_HIP_OK, back = -1;
-    bool capturing = false;
     explicit OnStream(void* stream) {
         DeviceState* st = state();
         if (!st) {
@@ -109,14 +134,17 @@ struct OnStream {
         int cur = -1;
         if (hipGetDevice(&cur) == hipSuccess && cur != st->device && hipSetDevice(st->device) == hipSuccess) back = cur;
         s = stream ? static_cast<hipStream_t>(stream) : cur_stream();
-        hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
-        capturing = hipStreamIsCapturing(s, &cs) == hipSuccess && cs != hipStreamCaptureStatusNone;
-        (void)hipGetLastError();
-        if (capturing && note_stream_syncs(s)) {
+        if (note_stream_syncs(s) && capturing()) {
             rc = arg_error("the first library call on a caller stream cannot be captured; make one call on that stream before capturing it");
             return;
         }
         note_stream(s);
+    }
+    bool capturing() const {
+        hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+        const bool yes = hipStreamIsCapturing(s, &cs) == hipSuccess && cs != hipStreamCaptureStatusNone;
+        (void)hipGetLastError();
+        return yes;
     }
     ~OnStream() {
         if (back >= 0) (void)hipSetDevice(back);
@@ -137,12 +165,13 @@ static int attend(PagedAttn a, int q_dtype, int kv_dtype, void* workspace, size_
     }
     OnStream on(stream);
     if (on.rc) return on.rc;
-    if (!workspace && on.capturing) return arg_error("a captured call needs a workspace of the caller's");
+    const bool capturing = on.capturing();
+    if (!workspace && capturing) return arg_error("a captured call needs a workspace of the caller's");
     void* ws = workspace ? workspace : dev_alloc_on(need, on.s);
     if (!ws) return TL_HIP_ERR_ALLOC;
     a.ws = static_cast<float*>(ws);
     // the arrival counters are the device's: only while calls cannot overlap, and not in a graph
-    a.fuse = single_stream() && one_launch_merge() && !on.capturing;
+    a.fuse = single_stream() && one_launch_merge() && !capturing;
     const int rc = launch_paged_attention(a, q_dtype == TL_HIP_F16, kv_dtype == TL_HIP_F16, on.s);
     if (!workspace) dev_free_on(ws, on.s);
     return rc;
@@ -205,13 +234,16 @@ int tl_hip_launch_kv_append(const void* k_new, const void* v_new, int new_dtype,
     a.kn = k_new, a.vn = v_new, a.ks = k_row_stride, a.vs = v_row_stride;
     OnStream on(stream);
     if (on.rc) return on.rc;
-    const int64_t units = n_tokens * 2 * width / 8;
-    const dim3 grid((unsigned)cdiv(units, 256));
+    // few rows: one per workgroup, for their latency
     const bool n16 = new_dtype == TL_HIP_F16, c16 = kv_dtype == TL_HIP_F16;
-    if (n16 && c16) k_kv_append<_Float16, _Float16><<<grid, 256, 0, on.s>>>(a);
-    else if (n16) k_kv_append<_Float16, float><<<grid, 256, 0, on.s>>>(a);
-    else if (c16) k_kv_append<float, _Float16><<<grid, 256, 0, on.s>>>(a);
-    else k_kv_append<float, float><<<grid, 256, 0, on.s>>>(a);
+#define TLH_APPEND(NT, KVT)                                                                                                \
+    (n_tokens <= 512 ? k_kv_append<NT, KVT, 1><<<dim3((unsigned)n_tokens), 256, 0, on.s>>>(a, page_table, cu_seqlens, kv_lens) \
+                     : k_kv_append<NT, KVT, 4><<<dim3((unsigned)cdiv(n_tokens, 4)), 256, 0, on.s>>>(a, page_table, cu_seqlens, kv_lens))
+    if (n16 && c16) TLH_APPEND(_Float16, _Float16);
+    else if (n16) TLH_APPEND(_Float16, float);
+    else if (c16) TLH_APPEND(float, _Float16);
+    else TLH_APPEND(float, float);
+#undef TLH_APPEND
     return launched("append launch");
 }
 
@@ -246,7 +278,7 @@ int tl_hip_launch_kv_copy_pages(void* k_pages, void* v_pages, int64_t n_layers, 
     OnStream on(stream);
     if (on.rc) return on.rc;
     CopyArgs a;
-    a.k = static_cast<uint4*>(k_pages), a.v = static_cast<uint4*>(v_pages);
+    a.k = static_cast<u32x4*>(k_pages), a.v = static_cast<u32x4*>(v_pages);
     a.page = page_bytes / 16, a.layer = n_pages * a.page;
     for (int64_t i0 = 0; i0 < n_pairs; i0 += COPY_PAIRS) {
         const int n = (int)std::min<int64_t>(COPY_PAIRS, n_pairs - i0);

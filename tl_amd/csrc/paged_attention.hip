@@ -24,50 +24,6 @@ typedef _Float16 half4v __attribute__((ext_vector_type(4)));
 // adds them in order.
 constexpr int RUNS = 512;  // at most: two workgroups per CU
 
-// Sequences base + lane: packed rows first .. first + n - 1, positions len that the table holds,
-// and `shown` positions that its row 0 sees (0 or fewer: none).
-struct Seq {
-    int first, n, len, shown;
-};
-// Groups are loaded in order from 0: a sequence's rows begin behind those of all before it, so
-// that they never add up to more than the call's, whatever cu holds.
-struct Group {
-    Seq q;
-    int base, reach;  // reach: the end of the rows of this group and those before
-    __device__ __forceinline__ void load(const PagedCache& c, const int32_t* cu, const int32_t* lens, int from) {
-        const int behind = from == 0 ? 0 : reach;
-        base = from;
-        const int b = from + (int)__lane_id();
-        int n = 0, lo = 0, hi = 0;
-        if (b < c.batch) {
-            n = lens[b], lo = b, hi = b + 1;  // (requested together)
-            if (cu) lo = cu[b], hi = cu[b + 1];
-        }
-        lo = min(max(lo, 0), c.rows), hi = min(max(hi, 0), c.rows), n = min(max(n, 0), INT32_MAX - 32);
-        if (cu) {
-            int top = max(hi, behind);
-#pragma unroll
-            for (int off = 1; off < 64; off <<= 1) top = max(top, __shfl_up(top, off));  // (lanes below off get their own)
-            const int before = __shfl_up(top, 1);
-            lo = max(lo, __lane_id() ? before : behind);
-            reach = __builtin_amdgcn_readlane(top, 63);
-        }
-        q.first = lo, q.n = max(hi - lo, 0), q.len = min(n, c.capacity), q.shown = n - q.n + 1;
-    }
-    __device__ __forceinline__ Seq at(int b) const {
-        const int i = b - base;
-        return Seq{__builtin_amdgcn_readlane(q.first, i), __builtin_amdgcn_readlane(q.n, i), __builtin_amdgcn_readlane(q.len, i),
-                   __builtin_amdgcn_readlane(q.shown, i)};
-    }
-    // the same, from a later group where b lies there
-    __device__ __forceinline__ Seq at(const PagedCache& c, const int32_t* cu, const int32_t* lens, int b) {
-        while (b - base >= 64) load(c, cu, lens, base + 64);
-        return at(b);
-    }
-};
-// Positions that row i of a sequence sees.
-__device__ __forceinline__ int limit_of(const Seq& q, int i) { return max(min(q.shown + i, q.len), 0); }
-
 struct Work {
     int tiles, rounds;
 };
@@ -212,7 +168,7 @@ struct Tile {
 
 // FULL: head_dim is DP (otherwise the rest of a key's pieces are zeros; the rest of a value's
 // make rows of the product that are not stored, and read the row's first elements).
-template <typename KVT, typename QT, int DP, int TK, bool FULL>
+template <typename KVT, typename QT, int DP, int TK, bool FULL, bool PACKED>
 __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_tile(
     const PagedAttn a, const int32_t* __restrict__ table, const int32_t* __restrict__ cu, const int32_t* __restrict__ lens,
     const char* __restrict__ kp, const char* __restrict__ vp) {
@@ -237,7 +193,7 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_tile(
     const int runs = gridDim.x, id = blockIdx.x;
     const int run = (runs & 7) == 0 ? (id & 7) * (runs >> 3) + (id >> 3) : id;
 
-    Group grp;
+    Group<PACKED> grp;
     int64_t total = 0, incl = 0, mine = 0;
     for (int base = 0; base < c.batch; base += 64) {
         grp.load(c, cu, lens, base);
@@ -659,7 +615,7 @@ struct Prompt {
 __device__ __forceinline__ bool prompt_tile(const PagedCache& c, const int32_t* cu, const int32_t* lens, int G, int shift, int index,
                                             bool cut, bool whole_units, Prompt* p) {
     const int up = (1 << shift) - 1;
-    Group grp;
+    Group<true> grp;
     int64_t total = 0, incl = 0, mine = 0;
     for (int base = 0; base < c.batch; base += 64) {
         grp.load(c, cu, lens, base);
@@ -1181,12 +1137,12 @@ __global__ __launch_bounds__(256) void k_prompt_join(const PagedAttn a, const in
 
 // The join, one workgroup per (sequence, KV head, tile) that there can be, in the line's order:
 // for calls whose parts are not joined where they were made.
-template <typename QT>
+template <typename QT, bool PACKED>
 __global__ __launch_bounds__(256) void k_paged_join(const PagedAttn a, const int32_t* __restrict__ cu, const int32_t* __restrict__ lens, int keys, int runs) {
     __shared__ __attribute__((aligned(16))) float room[JOIN_ROOM];
     const PagedCache& c = a.c;
     const int G = a.G;
-    Group grp;
+    Group<PACKED> grp;
     Seq sq{};
     int64_t total = 0, units = 0, at = -1, nth = 0;
     int b = -1;
@@ -1243,17 +1199,22 @@ size_t paged_attention_workspace(int64_t batch, int64_t rows, int hq, int hkv, i
     return most * (D + 4) * sizeof(float);
 }
 
-template <typename KVT, typename QT, int DP, int TK, bool FULL>
-static int launch_tile_of(const PagedAttn& a, hipStream_t s) {
+template <typename KVT, typename QT, int DP, int TK, bool FULL, bool PACKED>
+static int launch_runs(const PagedAttn& a, hipStream_t s) {
     constexpr int KEYS = Tile<KVT, QT, DP, TK>::KEYS;
     // as many runs as there can be rounds, up to two workgroups per CU
-    const int64_t units = a.c.cu ? units_of(a.c.batch, a.c.rows, a.G, a.c.hkv, 16) : (int64_t)a.c.hkv * a.c.batch * cdiv(a.G, 16);
+    const int64_t units = PACKED ? units_of(a.c.batch, a.c.rows, a.G, a.c.hkv, 16) : (int64_t)a.c.hkv * a.c.batch * cdiv(a.G, 16);
     const int64_t most = units * cdiv(a.c.capacity, KEYS);
     const int runs = (int)(most < RUNS ? most : RUNS);
-    k_paged_tile<KVT, QT, DP, TK, FULL><<<dim3((unsigned)runs), 256, 0, s>>>(a, a.c.table, a.c.cu, a.c.lens, static_cast<const char*>(a.c.k), static_cast<const char*>(a.c.v));
-    if (!a.fuse) k_paged_join<QT><<<dim3((unsigned)units), 256, 0, s>>>(a, a.c.cu, a.c.lens, KEYS, runs);
+    k_paged_tile<KVT, QT, DP, TK, FULL, PACKED><<<dim3((unsigned)runs), 256, 0, s>>>(a, a.c.table, a.c.cu, a.c.lens, static_cast<const char*>(a.c.k), static_cast<const char*>(a.c.v));
+    if (!a.fuse) k_paged_join<QT, PACKED><<<dim3((unsigned)units), 256, 0, s>>>(a, a.c.cu, a.c.lens, KEYS, runs);
     hipError_t e = hipGetLastError();
     return e == hipSuccess ? TL_HIP_OK : hip_fail(e, "paged attention launch");
+}
+
+template <typename KVT, typename QT, int DP, int TK, bool FULL>
+static int launch_tile_of(const PagedAttn& a, hipStream_t s) {
+    return a.c.cu ? launch_runs<KVT, QT, DP, TK, FULL, true>(a, s) : launch_runs<KVT, QT, DP, TK, FULL, false>(a, s);
 }
 
 template <typename KVT, typename QT, int DP, int TK>
