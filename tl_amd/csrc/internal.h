@@ -53,6 +53,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buf_rsrc(const void* p, uint32
 // Cache policy of a buffer access that is coherent at agent scope (the sc1 bit): the policy of
 // agent-scope atomic loads and stores on this target.
 constexpr int CPOL_SC1 = 16;
+constexpr int CPOL_NT = 2;  // non-temporal
 __device__ __forceinline__ uint4 ld_stream(const uint4* p) {
     const u32x4 t = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
     return uint4{t.x, t.y, t.z, t.w};

@@ -24,6 +24,14 @@ typedef _Float16 half4v __attribute__((ext_vector_type(4)));
 // adds them in order.
 constexpr int RUNS = 512;  // at most: two workgroups per CU
 
+// A sequence's row of the page table, in the constant address space: no kernel writes it, and its
+// entries are the same for a wavefront, so they come by scalar loads.  (As vector loads the wait
+// for a page number was a wait for all the keys and values requested before it.)
+typedef const __attribute__((address_space(4))) int32_t* table_ptr;
+__device__ __forceinline__ table_ptr table_row(const int32_t* table, const PagedCache& c, int b) {
+    return (table_ptr)(uintptr_t)(table + (int64_t)b * c.table_stride);
+}
+
 struct Work {
     int tiles, rounds;
 };
@@ -45,7 +53,9 @@ __device__ __forceinline__ int64_t lane_prefix(int64_t v) {
     return v;
 }
 __device__ __forceinline__ int64_t run_length(int64_t total, int runs) {
-    return total <= runs ? 1 : total <= 0x7FFFFFFF ? ((uint32_t)total + runs - 1) / (uint32_t)runs : (total + runs - 1) / runs;
+    const int64_t up = total + runs - 1;
+    const int64_t n = (runs & (runs - 1)) == 0 ? up >> __builtin_ctz(runs) : up <= 0x7FFFFFFF ? (uint32_t)up / (uint32_t)runs : up / runs;
+    return n < 1 ? 1 : n;
 }
 __device__ __forceinline__ uint32_t div_u(int64_t a, int64_t b) {
     if (((a | b) >> 32) == 0) return (uint32_t)a / (uint32_t)b;
@@ -246,16 +256,16 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_tile(
         const uint32_t unit = __builtin_amdgcn_readfirstlane(div_u(x - before, w.rounds));
         const int r0 = __builtin_amdgcn_readfirstlane((int)(x - before - (int64_t)unit * w.rounds));
         const int r1 = __builtin_amdgcn_readfirstlane((int)min((int64_t)w.rounds, r0 + (x1 - x)));
-        const int h = unit / w.tiles, tile = unit - h * w.tiles;
+        const int h = w.tiles == 1 ? unit : unit / w.tiles, tile = unit - h * w.tiles;
         const int64_t begin = x - r0;
         x += r1 - r0;
 
         // this lane's row; positions that it, that every row and that any row sees
         const int rows = sq.n * G;
-        const int r = min(tile * 16 + col, rows - 1), qi = r / G, qh = h * G + r - qi * G;
+        const int r = min(tile * 16 + col, rows - 1), qi = PACKED ? r / G : 0, qh = h * G + r - qi * G;
         const int lim = limit_of(sq, qi);
-        const int lim_lo = __builtin_amdgcn_readfirstlane(limit_of(sq, tile * 16 / G));
-        const int lim_hi = __builtin_amdgcn_readfirstlane(limit_of(sq, min(tile * 16 + 15, rows - 1) / G));
+        const int lim_lo = __builtin_amdgcn_readfirstlane(limit_of(sq, PACKED ? tile * 16 / G : 0));
+        const int lim_hi = __builtin_amdgcn_readfirstlane(limit_of(sq, PACKED ? min(tile * 16 + 15, rows - 1) / G : 0));
 
         const QT* qp = static_cast<const QT*>(a.q) + (int64_t)(sq.first + qi) * a.q_stride + qh * D;
         constexpr int QV = sizeof(QT) * L::PIECE / 16;  // 16-byte words per piece of the row
@@ -273,9 +283,7 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_tile(
         const int j_first = r0 * KEYS + wave * 16 * TK;
         const int j_end = min(r1 * KEYS, lim_hi);
         const int steps = j_first < j_end ? (j_end - j_first + KEYS - 1) / KEYS : 0;
-        const int32_t* row = table + (int64_t)b * c.table_stride;
-        // the block's positions in whole 16s, those past the last one seen moved back onto it
-        auto base16 = [&](int j) { return max(min(j, (lim_hi - 1) & ~15), 0); };
+        const table_ptr row = table_row(table, c, b);
         struct Ids {
             int p[TK];
         };
@@ -283,7 +291,7 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_tile(
             Ids d;
 #pragma unroll
             for (int t = 0; t < TK; t++)
-                d.p[t] = __builtin_amdgcn_readfirstlane(row[base16(j_first + s * KEYS + 16 * t) >> c.shift]);
+                d.p[t] = row[__builtin_amdgcn_readfirstlane(max(min(j_first + s * KEYS + 16 * t, lim_hi - 1), 0) >> c.shift)];
             return d;
         };
         struct Buf {
@@ -292,36 +300,40 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_tile(
         };
         const uint32_t kof = (uint32_t)(col * D + L::PIECE * g) * EB;  // + 64 s bytes
         const uint32_t vof = (uint32_t)(4 * g * D + VE * col) * EB;    // + e D EB + 16 VE i EB
-        uint32_t vofs[VN];
+        [[maybe_unused]] uint32_t kofs[KS], vofs[VN];
+        if constexpr (!FULL) {
 #pragma unroll
-        for (int i = 0; i < VN; i++) vofs[i] = 16 * VE * i + VE * col < D ? vof + 16 * VE * i * EB : (uint32_t)(4 * g * D) * EB;
+            for (int i = 0; i < KS; i++) kofs[i] = 4 * L::PIECE * i + L::PIECE * g < D ? kof + 64 * i : 0x7FFFFFF0u;
+#pragma unroll
+            for (int i = 0; i < VN; i++) vofs[i] = 16 * VE * i + VE * col < D ? vof + 16 * VE * i * EB : (uint32_t)(4 * g * D) * EB;
+        }
+        // a block's 16 keys lie in one page; keys past the last one seen, and blocks past the last
+        // step's, lie outside the resources and read as zeros, without a memory access
         auto load = [&](int s, const Ids& d, Buf& f) __attribute__((always_inline)) {
 #pragma unroll
             for (int t = 0; t < TK; t++) {
-                const int j = base16(j_first + s * KEYS + 16 * t);
-                const int p = (uint32_t)d.p[t] < (uint32_t)c.n_pages ? d.p[t] : 0;
-                const int64_t at = (p * c.page_elems + (int64_t)(j & (page - 1)) * D) * EB + head;
-                const char *kb = kp + at, *vb = vp + at;
+                const int j = j_first + s * KEYS + 16 * t;
+                const bool none = (uint32_t)d.p[t] >= (uint32_t)c.n_pages;
+                const int64_t at = ((none ? 0 : d.p[t]) * c.page_elems + (int64_t)(j & (page - 1)) * D) * EB + head;
+                const uint32_t bytes = (uint32_t)__builtin_amdgcn_readfirstlane(none || s >= steps ? 0 : max(min(lim_hi - j, 16), 0) * D * EB);
+                const __amdgpu_buffer_rsrc_t rk = buf_rsrc(kp + at, bytes), rv = buf_rsrc(vp + at, bytes);
 #pragma unroll
-                for (int i = 0; i < KS; i++) {
-                    if (FULL || 4 * L::PIECE * (i + 1) <= D) {
-                        f.k[t][i] = __builtin_nontemporal_load(reinterpret_cast<const piece*>(kb + kof + 64 * i));
-                    } else {
-                        f.k[t][i] = piece{};
-                        if (4 * L::PIECE * i + L::PIECE * g < D) f.k[t][i] = __builtin_nontemporal_load(reinterpret_cast<const piece*>(kb + kof + 64 * i));
-                    }
-                }
+                for (int i = 0; i < KS; i++)
+                    f.k[t][i] = __builtin_bit_cast(piece, __builtin_amdgcn_raw_buffer_load_b128(rk, FULL ? kof + 64 * i : kofs[i], 0, CPOL_NT));
 #pragma unroll
                 for (int e = 0; e < 4; e++)
 #pragma unroll
-                    for (int i = 0; i < VN; i++)
-                        f.v[4 * t + e][i] = __builtin_nontemporal_load(reinterpret_cast<const vec*>(vb + (FULL ? vof + 16 * VE * i * EB : vofs[i]) + e * D * EB));
+                    for (int i = 0; i < VN; i++) {
+                        const uint32_t o = (FULL ? vof + 16 * VE * i * EB : vofs[i]) + e * D * EB;
+                        if constexpr (sizeof(vec) == 8) f.v[4 * t + e][i] = __builtin_bit_cast(vec, __builtin_amdgcn_raw_buffer_load_b64(rv, o, 0, CPOL_NT));
+                        else f.v[4 * t + e][i] = __builtin_bit_cast(vec, __builtin_amdgcn_raw_buffer_load_b128(rv, o, 0, CPOL_NT));
+                    }
             }
         };
         Buf f0, f1;
-        Ids d0 = ids_of(0), d1 = ids_of(max(min(1, steps - 1), 0));
+        Ids d0 = ids_of(0), d1 = ids_of(1);
         __builtin_amdgcn_sched_barrier(0);
-        load(0, d0, f0);  // (without steps too: a wait for the query does not wait for these then)
+        load(0, d0, f0);
         __builtin_amdgcn_sched_barrier(0);
 
         float cs = fminf(fabsf(a.scale) * 1.44269504088896341f, FLT_MAX);
@@ -383,25 +395,18 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_tile(
             for (int t = 0; t < TK; t++) odd |= (uint32_t)d.p[t] >= (uint32_t)c.n_pages;
             const bool edge = j0 + 16 * TK > lim_lo;
             bool fix = false;
-            if (edge || odd) {
+            if (__builtin_expect(edge || odd, 0)) {
 #pragma unroll
                 for (int t = 0; t < TK; t++) {
                     const bool none = (uint32_t)d.p[t] >= (uint32_t)c.n_pages;
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        const int j = j0 + 16 * t + 4 * g + e;
-                        if (none) st[t][e] = NAN;
-                        if (j >= lim) st[t][e] = -INFINITY;
-                        // values that no row sees (or of no page) are zeros: a weight of 0 would
-                        // not silence an infinity
-                        if (none || j >= lim_hi) {
-#pragma unroll
-                            for (int i = 0; i < VN; i++) f.v[4 * t + e][i] = vec{};
-                        }
+                        if (none) st[t][e] = NAN;  // (over values of zero)
+                        if (j0 + 16 * t + 4 * g + e >= lim) st[t][e] = -INFINITY;
                     }
                 }
-                // those that only some rows see: infinities and NaN are taken out of the product
-                // and added to the rows that see them
+                // values that only some rows see: a weight of 0 would not silence an infinity.
+                // Infinities and NaN are taken out of the product and added to the rows that see them
                 if (lim_lo < lim_hi) {
                     uint32_t wild = 0;
 #pragma unroll
@@ -483,7 +488,7 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_tile(
                             for (int y = 0; y < VE; y++)
                                 acc[i * VE + y] = __builtin_amdgcn_mfma_f32_16x16x4f32(f.v[4 * t + e][i][y], st[t][e], acc[i * VE + y], 0, 0, 0);
             }
-            if (fix) {
+            if (__builtin_expect(fix, 0)) {
 #pragma unroll 1
                 for (int k = 0; k < 16 * TK; k++) {
                     int dims = D;
@@ -505,26 +510,20 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_tile(
             }
         };
 
-        // the next block's loads are in flight under this one's work; no load is conditional
-        // inside the loop, or the waits would count for the path without it
-        if (steps > 0) {
-            int s = 0;
-            for (; s + 2 < steps; s += 2) {
-                load(s + 1, d1, f1);
-                __builtin_amdgcn_sched_barrier(0);
-                const Ids d2 = ids_of(s + 2), d3 = ids_of(min(s + 3, steps - 1));
-                compute(s, d0, f0);
-                __builtin_amdgcn_sched_barrier(0);
-                load(s + 2, d2, f0);
-                __builtin_amdgcn_sched_barrier(0);
-                compute(s + 1, d1, f1);
-                __builtin_amdgcn_sched_barrier(0);
-                d0 = d2, d1 = d3;
-            }
-            if (s + 1 < steps) load(s + 1, d1, f1);
+        // the next block's loads are in flight under this one's work; none is conditional, or the
+        // waits would count for the path without it
+        for (int s = 0; s < steps; s += 2) {
+            load(s + 1, d1, f1);
             __builtin_amdgcn_sched_barrier(0);
+            const Ids d2 = ids_of(s + 2), d3 = ids_of(s + 3);
             compute(s, d0, f0);
-            if (s + 1 < steps) compute(s + 1, d1, f1);
+            __builtin_amdgcn_sched_barrier(0);
+            if (s + 1 >= steps) break;
+            load(s + 2, d2, f0);
+            __builtin_amdgcn_sched_barrier(0);
+            compute(s + 1, d1, f1);
+            __builtin_amdgcn_sched_barrier(0);
+            d0 = d2, d1 = d3;
         }
         l = lane_pair_sum<16>(l);
         l = lane_pair_sum<32>(l);
@@ -551,7 +550,7 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_tile(
 #pragma unroll
         for (int v = 0; v < 4; v++) fw[v] = __builtin_amdgcn_exp2f((so[v][tr][DP] - Ms) * rc), sum = fmaf(so[v][tr][DP + 1], fw[v], sum);
         const bool whole = r0 == 0 && r1 == w.rounds;
-        const int orow = tile * 16 + tr, oq = orow / G;
+        const int orow = tile * 16 + tr, oq = PACKED ? orow / G : 0;
         const uint32_t rec = (uint32_t)(2 * run + (r0 == 0 ? 1 : 0)) * (16 * (D + 4) * 4) + tr * (D + 4) * 4;  // bytes
         const __amdgpu_buffer_rsrc_t ws = buf_rsrc(a.ws, RUNS * 2 * 16 * (D + 4) * 4);
         const int sees = sq.shown + oq;
@@ -753,9 +752,9 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_prompt(
         ko[u] = 8 * ck < D ? (uint32_t)(rr * D + 8 * ck) * 2 : 0x7FFFFFF0u;
         vo[u] = 8 * cv < D ? (uint32_t)(rr * D + 8 * cv) * 2 : 0x7FFFFFF0u;
     }
-    const int32_t* row = table + (int64_t)b * c.table_stride;
+    const table_ptr row = table_row(table, c, b);
     const int64_t head = (int64_t)h * page * D;
-    auto page_of = [&](int j0) { return uniform(row[max(min(j0 + wave * RPW, last - 1), 0) >> c.shift]); };
+    auto page_of = [&](int j0) { return row[uniform(max(min(j0 + wave * RPW, last - 1), 0) >> c.shift)]; };
     auto issue = [&](int j0, int pid, Stage& st) __attribute__((always_inline)) {
         const int j = j0 + wave * RPW;
         const bool none = (uint32_t)pid >= (uint32_t)c.n_pages;
@@ -973,9 +972,9 @@ __global__ __launch_bounds__(256, 2) void k_paged_prompt_f32(
         ko[u] = 4 * ck < D ? (uint32_t)(rr * D + 4 * ck) * 4 : 0x7FFFFFF0u;
         vo[u] = 4 * ch < D ? (uint32_t)(rr * D + 4 * ch) * 4 : 0x7FFFFFF0u;
     }
-    const int32_t* row = table + (int64_t)b * c.table_stride;
+    const table_ptr row = table_row(table, c, b);
     const int64_t head = (int64_t)h * page * D;
-    auto page_of = [&](int j0) { return uniform(row[max(min(j0 + wave * RPW, last - 1), 0) >> c.shift]); };
+    auto page_of = [&](int j0) { return row[uniform(max(min(j0 + wave * RPW, last - 1), 0) >> c.shift)]; };
     auto issue = [&](int j0, int pid, Stage& st) __attribute__((always_inline)) {
         const int j = j0 + wave * RPW;
         const bool none = (uint32_t)pid >= (uint32_t)c.n_pages;
