@@ -39,27 +39,22 @@ __device__ __forceinline__ Work work_of(const Seq& q, int G, int keys) {
     if (q.n == 0) return {0, 0};
     return {(q.n * G + 15) >> 4, (q.len + keys - 1) / keys};
 }
-__device__ __forceinline__ int64_t lane_value(int64_t v, int lane) {
-    return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)v, lane) |
-                     (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32);
-}
-// sum over lanes 0 .. this one
-__device__ __forceinline__ int64_t lane_prefix(int64_t v) {
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const int64_t o = __shfl_up(v, off);
-        if ((int)__lane_id() >= off) v += o;
-    }
+// The line's length fits 31 bits (the launch sees to it).  Sum over lanes 0 .. this one: within 16
+// lanes, then lane 15's over the next row, then lane 31's over the upper half.
+__device__ __forceinline__ int lane_prefix(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);  // row_shr:1
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2 and 3
     return v;
 }
-__device__ __forceinline__ int64_t run_length(int64_t total, int runs) {
-    const int64_t up = total + runs - 1;
-    const int64_t n = (runs & (runs - 1)) == 0 ? up >> __builtin_ctz(runs) : up <= 0x7FFFFFFF ? (uint32_t)up / (uint32_t)runs : up / runs;
+__device__ __forceinline__ int lane_value(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+__device__ __forceinline__ int run_length(int total, int runs) {
+    const uint32_t up = (uint32_t)total + runs - 1;
+    const int n = (runs & (runs - 1)) == 0 ? up >> __builtin_ctz(runs) : up / (uint32_t)runs;
     return n < 1 ? 1 : n;
-}
-__device__ __forceinline__ uint32_t div_u(int64_t a, int64_t b) {
-    if (((a | b) >> 32) == 0) return (uint32_t)a / (uint32_t)b;
-    return (uint32_t)((uint64_t)a / (uint64_t)b);
 }
 
 // All ones over the f32 or the two f16 of a word that are infinite or NaN, else 0.
@@ -73,8 +68,8 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
 // Adds the parts of a tile's records, in order, and writes its rows: part 0 at byte `first` of the
 // workspace, part i at rest + i step.  A thread per four elements, over all parts or, where the rows are few, over every `slices`-th
 // and then over the slices.  Eight parts are requested at a time.
-constexpr int JOIN_ROOM = 256 * 7;  // floats of LDS
-template <typename QT, int POLICY>
+constexpr int JOIN_ROOM = 7;  // floats of LDS per thread
+template <typename QT, int POLICY, int NT>  // NT threads
 __device__ __forceinline__ void join_tile(const PagedAttn& a, const Seq& sq, int h, int tile, uint32_t first, uint32_t rest,
                                           uint32_t step, int parts, uint32_t bytes, float* room) {
     const int G = a.G, D = a.c.D, R = min(16, sq.n * G - tile * 16), per = D / 4;
@@ -83,7 +78,7 @@ __device__ __forceinline__ void join_tile(const PagedAttn& a, const Seq& sq, int
     auto part = [&](int i) { return i == 0 ? first : rest + (uint32_t)i * step; };
     auto word4 = [&](uint32_t at) { return __builtin_bit_cast(floatx4, __builtin_amdgcn_raw_buffer_load_b128(ws, at, 0, POLICY)); };
     floatx4* po = reinterpret_cast<floatx4*>(room);
-    float *pm = room + 1024, *pl = room + 1280;
+    float *pm = room + 4 * NT, *pl = room + 5 * NT, *pc = room + 6 * NT;
     struct Sum {
         floatx4 o;
         float m, l, cs;
@@ -96,7 +91,7 @@ __device__ __forceinline__ void join_tile(const PagedAttn& a, const Seq& sq, int
 #pragma unroll
         for (int e = 0; e < 4; e++) t.o[e] = fmaf(t.o[e], f, o[e] * g);
     };
-    const int items = R * per, slices = max(256 / items, 1);
+    const int items = R * per, slices = max(NT / items, 1);
     auto put = [&](int it, const Sum& t) {
         const int r = it / per, dim = 4 * (it - r * per), orow = tile * 16 + r, oq = orow / G, sees = sq.shown + oq;
         floatx4 o = t.o * (sees > sq.len ? NAN : 1.0f / t.l);
@@ -106,7 +101,7 @@ __device__ __forceinline__ void join_tile(const PagedAttn& a, const Seq& sq, int
         else *reinterpret_cast<half4v*>(op + dim) = half4v{(_Float16)o[0], (_Float16)o[1], (_Float16)o[2], (_Float16)o[3]};
     };
     const int slice = slices > 1 ? (int)threadIdx.x / items : 0;
-    for (int it = slices > 1 ? (int)threadIdx.x - slice * items : (int)threadIdx.x; it < items && slice < slices; it += 256) {
+    for (int it = slices > 1 ? (int)threadIdx.x - slice * items : (int)threadIdx.x; it < items && slice < slices; it += NT) {
         const int r = it / per;
         Sum t{{0.f, 0.f, 0.f, 0.f}, -INFINITY, 0.f, 1.f};
         for (int i0 = slice; i0 < parts; i0 += 8 * slices) {
@@ -129,23 +124,22 @@ __device__ __forceinline__ void join_tile(const PagedAttn& a, const Seq& sq, int
             put(it, t);
         } else {
             po[threadIdx.x] = t.o, pm[threadIdx.x] = t.m, pl[threadIdx.x] = t.l;
-            if (slice == 0) room[1536 + threadIdx.x] = t.cs;
+            if (slice == 0) pc[threadIdx.x] = t.cs;
         }
     }
     if (slices == 1) return;
     __syncthreads();
     const int it = threadIdx.x;
     if (it >= items) return;
-    Sum t{po[it], pm[it], pl[it], room[1536 + it]};
-    for (int i = 1; i < slices; i++)
-        if (i < parts) add(t, po[it + i * items], pm[it + i * items], pl[it + i * items]);
+    Sum t{po[it], pm[it], pl[it], pc[it]};
+    for (int i = 1; i < min(slices, parts); i++) add(t, po[it + i * items], pm[it + i * items], pl[it + i * items]);
     put(it, t);
 }
 // Runs run0 .. run0 + parts - 1 of k_paged_tile: the first run's record in its slot 1, the others' in slot 0.
-template <typename QT, int POLICY>
+template <typename QT, int POLICY, int NT>
 __device__ __forceinline__ void join_run(const PagedAttn& a, const Seq& sq, int h, int tile, int run0, int parts, float* room) {
     const uint32_t rec = 16 * (a.c.D + 4) * 4;
-    join_tile<QT, POLICY>(a, sq, h, tile, (2 * run0 + 1) * rec, 2 * run0 * rec, 2 * rec, parts, RUNS * 2 * rec, room);
+    join_tile<QT, POLICY, NT>(a, sq, h, tile, (2 * run0 + 1) * rec, 2 * run0 * rec, 2 * rec, parts, RUNS * 2 * rec, room);
 }
 // One launch: arrivals at the tile that run `i` began, zero between calls.  The run that arrives
 // last joins the tile and sets its counter back.
@@ -164,7 +158,7 @@ __device__ uint32_t g_paged_arrive[RUNS];
 // f16 caches: products exact in f32; f32 rows enter as two f16 parts (row scaled by a power of
 // two, 22 bits), weights as two parts of 2^15 p, so the results keep f32's digits.  f32 caches:
 // f32 matrix instructions.
-template <typename KVT, typename QT, int DP, int TK>
+template <typename KVT, typename QT, int DP, int TK, int NW>
 struct Tile {
     static constexpr bool H16 = std::is_same_v<KVT, _Float16>;
     static constexpr int QP = H16 && std::is_same_v<QT, float> ? 2 : 1;  // parts of a query
@@ -173,25 +167,25 @@ struct Tile {
     static constexpr int VE = DP / 16 < PIECE ? DP / 16 : PIECE;         // value elements per load
     static constexpr int VN = DP / 16 / VE;                              // loads per value row and lane
     static constexpr int NA = DP / 16;
-    static constexpr int KEYS = 64 * TK;  // positions per round
+    static constexpr int KEYS = 16 * TK * NW;  // positions per round
 };
 
 // FULL: head_dim is DP (otherwise the rest of a key's pieces are zeros; the rest of a value's
 // make rows of the product that are not stored, and read the row's first elements).
-template <typename KVT, typename QT, int DP, int TK, bool FULL, bool PACKED>
-__global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_tile(
+template <typename KVT, typename QT, int DP, int TK, int NW, bool FULL, bool PACKED>
+__global__ __launch_bounds__(64 * NW, (DP > 128 ? 1 : 2)) void k_paged_tile(
     const PagedAttn a, const int32_t* __restrict__ table, const int32_t* __restrict__ cu, const int32_t* __restrict__ lens,
     const char* __restrict__ kp, const char* __restrict__ vp) {
-    using L = Tile<KVT, QT, DP, TK>;
+    using L = Tile<KVT, QT, DP, TK, NW>;
     constexpr int QP = L::QP, KS = L::KS, VE = L::VE, VN = L::VN, NA = L::NA, KEYS = L::KEYS, EB = sizeof(KVT);
     constexpr bool H16 = L::H16;
     typedef KVT vec __attribute__((ext_vector_type(VE)));
     typedef uint32_t words __attribute__((ext_vector_type(sizeof(vec) / 4)));
     typedef KVT piece __attribute__((ext_vector_type(L::PIECE)));
     constexpr int RS = DP + 4;
-    __shared__ __attribute__((aligned(16))) float so[4][16][RS];  // o, then m, l and c
+    __shared__ __attribute__((aligned(16))) float so[NW][16][RS];  // o, then m, l and c
     __shared__ int last_here;
-    static_assert(sizeof(so) >= JOIN_ROOM * 4, "the join's room");
+    static_assert(sizeof(so) >= 64 * NW * JOIN_ROOM * 4, "the join's room");
     const PagedCache& c = a.c;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
     // arguments in one round of scalar loads (left to the compiler: three dependent rounds)
@@ -204,11 +198,11 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_tile(
     const int run = (runs & 7) == 0 ? (id & 7) * (runs >> 3) + (id >> 3) : id;
 
     Group<PACKED> grp;
-    int64_t total = 0, incl = 0, mine = 0;
+    int total = 0, incl = 0, mine = 0;
     for (int base = 0; base < c.batch; base += 64) {
         grp.load(c, cu, lens, base);
         const Work w = work_of(grp.q, G, KEYS);
-        mine = (int64_t)c.hkv * w.tiles * w.rounds;
+        mine = c.hkv * w.tiles * w.rounds;
         incl = lane_prefix(mine);
         total += lane_value(incl, 63);
         // rows of sequences without a position are zeros, and no round's
@@ -218,20 +212,20 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_tile(
             const Seq sq = grp.at(base + i);
             uint32_t* op = reinterpret_cast<uint32_t*>(static_cast<QT*>(a.out) + (int64_t)sq.first * a.hq * D);
             const int64_t words = (int64_t)sq.n * a.hq * D * (int)sizeof(QT) / 4;
-            for (int64_t u = threadIdx.x; u < words; u += 256) op[u] = 0;
+            for (int64_t u = threadIdx.x; u < words; u += 64 * NW) op[u] = 0;
         }
     }
-    const int64_t len_run = run_length(total, runs);
-    int64_t x = run * len_run;
-    const int64_t x1 = min(x + len_run, total);
-    if (x >= x1) return;
+    const int len_run = run_length(total, runs);
+    if ((int64_t)run * len_run >= total) return;
+    int x = run * len_run;
+    const int x1 = min(x + len_run, total);
     int b = 0;
-    int64_t before = 0;  // line position of sequence b's first round
+    int before = 0;  // line position of sequence b's first round
     for (int base = 0;; base += 64) {
         if (c.batch > 64) {
             grp.load(c, cu, lens, base);
             const Work w = work_of(grp.q, G, KEYS);
-            mine = (int64_t)c.hkv * w.tiles * w.rounds;
+            mine = c.hkv * w.tiles * w.rounds;
             incl = lane_prefix(mine);
         }
         const uint64_t hit = __ballot(x < before + incl);
@@ -247,17 +241,17 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_tile(
     while (x < x1) {
         const Seq sq = grp.at(c, cu, lens, b);
         const Work w = work_of(sq, G, KEYS);
-        const int64_t here = (int64_t)c.hkv * w.tiles * w.rounds;
+        const int here = c.hkv * w.tiles * w.rounds;
         if (x >= before + here) {
             before += here;
             b++;
             continue;
         }
-        const uint32_t unit = __builtin_amdgcn_readfirstlane(div_u(x - before, w.rounds));
-        const int r0 = __builtin_amdgcn_readfirstlane((int)(x - before - (int64_t)unit * w.rounds));
-        const int r1 = __builtin_amdgcn_readfirstlane((int)min((int64_t)w.rounds, r0 + (x1 - x)));
+        const uint32_t unit = __builtin_amdgcn_readfirstlane((uint32_t)(x - before) / (uint32_t)w.rounds);
+        const int r0 = __builtin_amdgcn_readfirstlane(x - before - (int)unit * w.rounds);
+        const int r1 = __builtin_amdgcn_readfirstlane(min(w.rounds, r0 + (x1 - x)));
         const int h = w.tiles == 1 ? unit : unit / w.tiles, tile = unit - h * w.tiles;
-        const int64_t begin = x - r0;
+        const int begin = x - r0;
         x += r1 - r0;
 
         // this lane's row; positions that it, that every row and that any row sees
@@ -539,16 +533,17 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_tile(
                     *reinterpret_cast<floatx4*>(&so[wave][col][16 * VE * i + VE * (4 * g + e) + y]) =
                         floatx4{acc[i * VE + y][e], acc[i * VE + y + 1][e], acc[i * VE + y + 2][e], acc[i * VE + y + 3][e]};
         __syncthreads();
-        // thread: row tr, every 16th float4 of it
-        const int tr = threadIdx.x >> 4, tc = threadIdx.x & 15;
+        // thread: row tr, every TPR-th float4 of it
+        constexpr int TPR = 4 * NW;
+        const int tr = threadIdx.x / TPR, tc = threadIdx.x % TPR;
         const float rc = so[0][tr][DP + 2];
         float M = -INFINITY;
 #pragma unroll
-        for (int v = 0; v < 4; v++) M = fmaxf(M, so[v][tr][DP]);
+        for (int v = 0; v < NW; v++) M = fmaxf(M, so[v][tr][DP]);
         const float Ms = M == -INFINITY ? 0.f : M;
-        float fw[4], sum = 0.f;
+        float fw[NW], sum = 0.f;
 #pragma unroll
-        for (int v = 0; v < 4; v++) fw[v] = __builtin_amdgcn_exp2f((so[v][tr][DP] - Ms) * rc), sum = fmaf(so[v][tr][DP + 1], fw[v], sum);
+        for (int v = 0; v < NW; v++) fw[v] = __builtin_amdgcn_exp2f((so[v][tr][DP] - Ms) * rc), sum = fmaf(so[v][tr][DP + 1], fw[v], sum);
         const bool whole = r0 == 0 && r1 == w.rounds;
         const int orow = tile * 16 + tr, oq = PACKED ? orow / G : 0;
         const uint32_t rec = (uint32_t)(2 * run + (r0 == 0 ? 1 : 0)) * (16 * (D + 4) * 4) + tr * (D + 4) * 4;  // bytes
@@ -558,12 +553,12 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_tile(
         QT* op = static_cast<QT*>(a.out) + ((int64_t)(sq.first + oq) * a.hq + h * G + orow - oq * G) * D;
         if (orow < rows) {
 #pragma unroll
-            for (int i = 0; i < (DP + 63) / 64; i++) {
-                const int dim = 64 * i + 4 * tc;
+            for (int i = 0; i < (DP + 4 * TPR - 1) / (4 * TPR); i++) {
+                const int dim = 4 * TPR * i + 4 * tc;
                 if (dim >= D) continue;
                 floatx4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int v = 0; v < 4; v++) {
+                for (int v = 0; v < NW; v++) {
                     const floatx4 z = *reinterpret_cast<const floatx4*>(&so[v][tr][dim]);
 #pragma unroll
                     for (int e = 0; e < 4; e++) o[e] = fmaf(z[e], fw[v], o[e]);
@@ -586,7 +581,7 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_tile(
             // one thread arrives; the records are read past the caches, after the arrival.
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
-            const int run0 = (int)div_u(begin, len_run), parts = (int)div_u(begin + w.rounds - 1, len_run) - run0 + 1;
+            const int run0 = (uint32_t)begin / (uint32_t)len_run, parts = (uint32_t)(begin + w.rounds - 1) / (uint32_t)len_run - run0 + 1;
             if (threadIdx.x == 0) {
                 const uint32_t old = __hip_atomic_fetch_add(&g_paged_arrive[run0], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 const bool end = old == (uint32_t)(parts - 1);
@@ -594,7 +589,7 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_tile(
                 last_here = end;
             }
             __syncthreads();
-            if (last_here) join_run<QT, CPOL_SC1>(a, sq, h, tile, run0, parts, &so[0][0][0]);
+            if (last_here) join_run<QT, CPOL_SC1, 64 * NW>(a, sq, h, tile, run0, parts, &so[0][0][0]);
         }
     }
 }
@@ -615,21 +610,21 @@ __device__ __forceinline__ bool prompt_tile(const PagedCache& c, const int32_t* 
                                             bool cut, bool whole_units, Prompt* p) {
     const int up = (1 << shift) - 1;
     Group<true> grp;
-    int64_t total = 0, incl = 0, mine = 0;
+    int total = 0, incl = 0, mine = 0;
     for (int base = 0; base < c.batch; base += 64) {
         grp.load(c, cu, lens, base);
         mine = (grp.q.n * G + up) >> shift;
         incl = lane_prefix(mine);
         total += lane_value(incl, 63);
     }
-    p->units = (int)(total * c.hkv);  // (rows and heads together are below 2^27)
+    p->units = total * c.hkv;  // (rows and heads together are below 2^27)
     if (p->units == 0) return false;
     p->most = cut ? max(SLOTS / p->units, 1) : 1;
     p->unit = cut && !whole_units ? index % p->units : index;
     if (p->unit >= p->units) return false;
     p->h = p->unit % c.hkv;
-    const int64_t nth = total - 1 - p->unit / c.hkv;
-    int64_t before = 0;
+    const int nth = total - 1 - p->unit / c.hkv;
+    int before = 0;
     for (int base = 0;; base += 64) {
         if (c.batch > 64) {
             grp.load(c, cu, lens, base);
@@ -640,7 +635,7 @@ __device__ __forceinline__ bool prompt_tile(const PagedCache& c, const int32_t* 
         if (hit) {
             const int at = __builtin_ctzll(hit);
             p->b = base + at;
-            p->tile = __builtin_amdgcn_readfirstlane((int)(nth - (before + lane_value(incl, at) - lane_value(mine, at))));
+            p->tile = __builtin_amdgcn_readfirstlane((nth - (before + lane_value(incl, at) - lane_value(mine, at))));
             break;
         }
         before += lane_value(incl, 63);
@@ -1120,7 +1115,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_prompt_f32(
 // Adds the parts of cut units, 16 rows to a workgroup.
 template <typename QT>
 __global__ __launch_bounds__(256) void k_prompt_join(const PagedAttn a, const int32_t* __restrict__ cu, const int32_t* __restrict__ lens, int shift, int keys) {
-    __shared__ __attribute__((aligned(16))) float room[JOIN_ROOM];
+    __shared__ __attribute__((aligned(16))) float room[256 * JOIN_ROOM];
     const PagedCache& c = a.c;
     const int G = a.G, per = 1 << (shift - 4), sub = blockIdx.x & (per - 1);
     Prompt pt;
@@ -1131,30 +1126,30 @@ __global__ __launch_bounds__(256) void k_prompt_join(const PagedAttn a, const in
     const int parts = prompt_parts(pt.most, (last + keys - 1) / keys);
     if (parts == 1) return;
     const uint32_t row = (c.D + 4) * 4, slot = row << shift, first = (uint32_t)(pt.unit * pt.most) * slot + 16 * sub * row;
-    join_tile<QT, 0>(a, pt.sq, pt.h, r0 >> 4, first, first, slot, parts, (uint32_t)SLOTS * slot, room);
+    join_tile<QT, 0, 256>(a, pt.sq, pt.h, r0 >> 4, first, first, slot, parts, (uint32_t)SLOTS * slot, room);
 }
 
 // The join, one workgroup per (sequence, KV head, tile) that there can be, in the line's order:
 // for calls whose parts are not joined where they were made.
-template <typename QT, bool PACKED>
-__global__ __launch_bounds__(256) void k_paged_join(const PagedAttn a, const int32_t* __restrict__ cu, const int32_t* __restrict__ lens, int keys, int runs) {
-    __shared__ __attribute__((aligned(16))) float room[JOIN_ROOM];
+template <typename QT, bool PACKED, int NT>
+__global__ __launch_bounds__(NT) void k_paged_join(const PagedAttn a, const int32_t* __restrict__ cu, const int32_t* __restrict__ lens, int keys, int runs) {
+    __shared__ __attribute__((aligned(16))) float room[NT * JOIN_ROOM];
     const PagedCache& c = a.c;
     const int G = a.G;
     Group<PACKED> grp;
     Seq sq{};
-    int64_t total = 0, units = 0, at = -1, nth = 0;
+    int total = 0, units = 0, at = -1, nth = 0;
     int b = -1;
     for (int base = 0; base < c.batch; base += 64) {
         grp.load(c, cu, lens, base);
         const Work w = work_of(grp.q, G, keys);
-        const int64_t wu = (int64_t)c.hkv * w.tiles, ww = wu * w.rounds, iu = lane_prefix(wu), iw = lane_prefix(ww);
-        const uint64_t hit = __ballot(blockIdx.x < units + iu);
+        const int wu = c.hkv * w.tiles, ww = wu * w.rounds, iu = lane_prefix(wu), iw = lane_prefix(ww);
+        const uint64_t hit = __ballot((int)blockIdx.x < units + iu);
         if (b < 0 && hit) {
             const int i = __builtin_ctzll(hit);
             b = base + i;
             sq = grp.at(b);
-            nth = blockIdx.x - (units + lane_value(iu, i) - lane_value(wu, i));
+            nth = (int)blockIdx.x - (units + lane_value(iu, i) - lane_value(wu, i));
             at = total + lane_value(iw, i) - lane_value(ww, i);
         }
         units += lane_value(iu, 63);
@@ -1163,11 +1158,11 @@ __global__ __launch_bounds__(256) void k_paged_join(const PagedAttn a, const int
     if (b < 0) return;
     const Work w = work_of(sq, G, keys);
     if (w.rounds == 0) return;
-    const int64_t len_run = run_length(total, runs), x = at + nth * w.rounds;
-    const int run0 = (int)div_u(x, len_run), run1 = (int)div_u(x + w.rounds - 1, len_run);
+    const uint32_t len_run = run_length(total, runs), x = at + nth * w.rounds;
+    const int run0 = x / len_run, run1 = (x + w.rounds - 1) / len_run;
     if (run0 == run1) return;
-    const int h = (int)div_u(nth, w.tiles), tile = (int)(nth - (int64_t)h * w.tiles);
-    join_run<QT, 0>(a, sq, h, tile, run0, run1 - run0 + 1, room);
+    const int h = (uint32_t)nth / (uint32_t)w.tiles, tile = nth - h * w.tiles;
+    join_run<QT, 0, NT>(a, sq, h, tile, run0, run1 - run0 + 1, room);
 }
 
 // Units that there can be, for tiles of `tile` rows.
@@ -1198,22 +1193,35 @@ size_t paged_attention_workspace(int64_t batch, int64_t rows, int hq, int hkv, i
     return most * (D + 4) * sizeof(float);
 }
 
-template <typename KVT, typename QT, int DP, int TK, bool FULL, bool PACKED>
-static int launch_runs(const PagedAttn& a, hipStream_t s) {
-    constexpr int KEYS = Tile<KVT, QT, DP, TK>::KEYS;
-    // as many runs as there can be rounds, up to two workgroups per CU
-    const int64_t units = PACKED ? units_of(a.c.batch, a.c.rows, a.G, a.c.hkv, 16) : (int64_t)a.c.hkv * a.c.batch * cdiv(a.G, 16);
-    const int64_t most = units * cdiv(a.c.capacity, KEYS);
-    const int runs = (int)(most < RUNS ? most : RUNS);
-    k_paged_tile<KVT, QT, DP, TK, FULL, PACKED><<<dim3((unsigned)runs), 256, 0, s>>>(a, a.c.table, a.c.cu, a.c.lens, static_cast<const char*>(a.c.k), static_cast<const char*>(a.c.v));
-    if (!a.fuse) k_paged_join<QT, PACKED><<<dim3((unsigned)units), 256, 0, s>>>(a, a.c.cu, a.c.lens, KEYS, runs);
+template <typename KVT, typename QT, int DP, int TK, int NW, bool FULL, bool PACKED>
+static int launch_runs(const PagedAttn& a, int64_t units, hipStream_t s) {
+    constexpr int KEYS = Tile<KVT, QT, DP, TK, NW>::KEYS;
+    // as many runs as there can be rounds, up to eight wavefronts per CU
+    const int64_t most = units * cdiv(a.c.capacity, KEYS), cap = RUNS * 4 / NW;
+    if (most > INT32_MAX - RUNS) {
+        set_error(TL_HIP_ERR_ARG, "ArgumentError: %lld rounds of %d positions are too many for one call", (long long)most, KEYS);
+        return TL_HIP_ERR_ARG;
+    }
+    const int runs = (int)(most < cap ? most : cap);
+    k_paged_tile<KVT, QT, DP, TK, NW, FULL, PACKED><<<dim3((unsigned)runs), 64 * NW, 0, s>>>(a, a.c.table, a.c.cu, a.c.lens, static_cast<const char*>(a.c.k), static_cast<const char*>(a.c.v));
+    if (!a.fuse) k_paged_join<QT, PACKED, 64 * NW><<<dim3((unsigned)units), 64 * NW, 0, s>>>(a, a.c.cu, a.c.lens, KEYS, runs);
     hipError_t e = hipGetLastError();
     return e == hipSuccess ? TL_HIP_OK : hip_fail(e, "paged attention launch");
 }
 
 template <typename KVT, typename QT, int DP, int TK, bool FULL>
 static int launch_tile_of(const PagedAttn& a, hipStream_t s) {
-    return a.c.cu ? launch_runs<KVT, QT, DP, TK, FULL, true>(a, s) : launch_runs<KVT, QT, DP, TK, FULL, false>(a, s);
+    if (a.c.cu) {
+        const int64_t units = units_of(a.c.batch, a.c.rows, a.G, a.c.hkv, 16);
+        return launch_runs<KVT, QT, DP, TK, 4, FULL, true>(a, units, s);
+    }
+    const int64_t units = (int64_t)a.c.hkv * a.c.batch * cdiv(a.G, 16);
+    // Few units over long tables: workgroups of eight wavefronts, so that half as many parts are
+    // joined.  us, against four: 8 units of 128 over 8192 positions 13.0 against 14.8, f32 caches of
+    // one unit 16.3 against 22.7; over 2048 12.2 against 9.4; 256 units up to 8192 95.6 against 92.2.
+    if constexpr (DP <= 128)
+        if (units < 128 && a.c.capacity >= 4096) return launch_runs<KVT, QT, DP, TK, 8, FULL, false>(a, units, s);
+    return launch_runs<KVT, QT, DP, TK, 4, FULL, false>(a, units, s);
 }
 
 template <typename KVT, typename QT, int DP, int TK>
