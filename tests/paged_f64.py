@@ -13,19 +13,23 @@ def positions(table, ps, pages, b, h, n):
 
 
 def attend(q, k, v, limit, scale):
-    """One query over rows 0 .. limit - 1 of k and v: (out, what one rounding per step may move)."""
+    """Queries [n, D] over rows 0 .. limit[i] - 1 of k and v: out, the error that one rounding per
+    step may make, and sum_j p_j |v_j|."""
     D = k.shape[1]
-    if limit <= 0:
-        return np.zeros(D), np.zeros(D), np.zeros(D)
-    q, k, v = q.astype(np.float64), k[:limit], v[:limit]
-    x = k @ q * scale
-    p = np.exp(x - x.max())
-    p /= p.sum()
+    seen = np.arange(len(k))[None] < limit[:, None]
+    some = limit > 0
+    q = q.astype(np.float64)
+    x = np.where(seen, q @ k.T * scale, -np.inf)
+    size = np.where(seen, np.abs(q) @ np.abs(k).T, 0.0)
+    top = np.where(some, np.max(x, axis=1, initial=-np.inf), 0.0)
+    p = np.exp(x - top[:, None])
+    p /= np.where(some, p.sum(1), 1.0)[:, None]
     # a score: D products and sums, the scale, and a query held in two parts of 11 bits (2^-22);
     # the exponential and its difference from the maximum: 16 steps
-    e = ((D + 16) * U32 + 2.0 ** -22) * abs(scale) * (np.abs(k) @ np.abs(q)).max() + 16 * U32 + np.abs(x - x.max()).max() * U32
+    far = np.max(np.where(seen, top[:, None] - x, 0.0), axis=1, initial=0.0)
+    e = ((D + 16) * U32 + 2.0 ** -22) * abs(scale) * size.max(1, initial=0.0) + 16 * U32 + far * U32
     near = p @ np.abs(v)
-    return p @ v, near * (2 * e + (limit + 64) * U32), near
+    return p @ v, near * (2 * e + (np.maximum(limit, 0) + 64) * U32)[:, None], near
 
 
 def attention(q, k_pages, v_pages, table, lens, cu, ps, scale, q16):
@@ -35,13 +39,11 @@ def attention(q, k_pages, v_pages, table, lens, cu, ps, scale, q16):
     out, tol = np.full(q.shape, np.nan), np.zeros(q.shape)
     for b in range(len(lens)):
         n = cu[b + 1] - cu[b]
-        for h in range(heads):
-            if not n:
-                continue
+        for h in range(heads if n else 0):
             k, v = positions(table, ps, k_pages, b, h // G, lens[b]), positions(table, ps, v_pages, b, h // G, lens[b])
-            for i in range(n):
-                o, t, near = attend(q[cu[b] + i, h], k, v, lens[b] - n + i + 1, scale)
-                # f16 rows: weights and result rounded to f16, half a step each (twice over, and
-                # f16's smallest steps below its normal numbers)
-                out[cu[b] + i, h], tol[cu[b] + i, h] = o, t + (U16 * (near + np.abs(o)) + 2.0 ** -24 * (near + 1) if q16 else 0)
+            at = slice(cu[b], cu[b + 1])
+            o, t, near = attend(q[at, h], k, v, lens[b] - n + 1 + np.arange(n), scale)
+            # f16 rows: weights and result rounded to f16, half a step each, and f16's smallest steps
+            # below its normal numbers
+            out[at, h], tol[at, h] = o, t + (U16 * (near + np.abs(o)) + 2.0 ** -24 * (near + 1) if q16 else 0)
     return out, tol

@@ -155,6 +155,50 @@ def test_prefill(dev, qt, kt, hkv, G, D, ps, new, past, extra):
 
 
 @pytest.mark.parametrize("qt,kt", TYPES)
+@pytest.mark.parametrize("hkv,G,D,ps,new,past,extra,room", [
+    (4, 4, 64, 16, [150, 1], [0, 700], 2, 16384),        # few tiles under a wide table: positions cut
+    (2, 4, 128, 64, [130, 0, 31], [900, 50, 0], 0, 32768),
+    (2, 7, 96, 32, [64], [1500], 1, 32768),
+    (1, 3, 256, 128, [200, 70], [333, 0], 0, 65536),
+    (1, 5, 136, 16, [90], [400], 0, 65536),
+    (1, 1, 40, 256, [300], [2000], 0, 65536),
+    (64, 4, 64, 64, [135], [60], 0, 0),                  # enough tiles to stay whole
+    (64, 4, 128, 16, [129, 2], [0, 33], 3, 0),
+    (66, 4, 80, 64, [128], [0], 0, 0),
+    (64, 2, 256, 32, [257], [20], 0, 0),
+])
+def test_prefill_of_long_prompts(dev, qt, kt, hkv, G, D, ps, new, past, extra, room):
+    lens = [n + p for n, p in zip(new, past)]
+    s = Setup(dev, 27 + D, lens, ps, hkv, D, kt, width=room // ps or None)
+    cu = np.concatenate([[0], np.cumsum(new)])
+    q = s.rng.standard_normal((cu[-1] + extra, hkv * G, D)).astype(qt)
+    scale = D ** -0.5
+    got = run_attention(s, q, scale, cu=cu)
+    check(got, *attention(q, s.k, s.v, s.table, lens, cu, ps, scale, qt == np.float16))
+    # what only later rows see, on whichever tile's edge it falls
+    b = int(np.argmax(new))
+    j = lens[b] - new[b] // 2
+    s.v[s.table[b, j // ps], :, j % ps, D // 2] = np.inf
+    s.k[s.table[b, (lens[b] - 1) // ps], :, (lens[b] - 1) % ps] = np.nan
+    again = run_attention(s, q, scale, cu=cu)
+    first = cu[b] + new[b] - new[b] // 2
+    assert not np.isfinite(again[first:cu[b + 1], :, D // 2]).any() and np.isnan(again[cu[b + 1] - 1]).all()
+    same = np.ones(got.shape, bool)
+    same[first:cu[b + 1], :, D // 2] = False
+    same[cu[b + 1] - 1] = False
+    assert np.array_equal(again[same], got[same])
+
+
+@pytest.mark.parametrize("qt,kt", TYPES)
+@pytest.mark.parametrize("hkv,G,D", [(2, 5, 64), (1, 8, 40), (1, 4, 80), (2, 16, 128)])
+def test_decode_of_few_long_sequences(dev, qt, kt, hkv, G, D):
+    lens = [5000, 0, 1, 4097]
+    s = Setup(dev, 28, lens, 32, hkv, D, kt)
+    q = s.rng.standard_normal((4, hkv * G, D)).astype(qt)
+    check(run_attention(s, q, 0.1), *attention(q, s.k, s.v, s.table, lens, range(5), 32, 0.1, qt == np.float16))
+
+
+@pytest.mark.parametrize("qt,kt", TYPES)
 def test_prefill_more_rows_than_positions(dev, qt, kt):
     """kv_lens below the number of rows: the first rows sit before position 0 and are zeros."""
     s = Setup(dev, 8, [20, 0], 16, 2, 64, kt)
@@ -376,6 +420,109 @@ def test_offsets_past_32_bits(dev):
             lib.tl_hip_free(p)
 
 
+def _stream(hip):
+    st = C.c_void_p()
+    assert hip.hipStreamCreateWithFlags(C.byref(st), 1) == 0   # hipStreamNonBlocking
+    return st
+
+
+@pytest.mark.parametrize("qt,kt", [(np.float32, F16), (np.float16, F16), (np.float32, F32)])
+def test_graphs_follow_the_lengths_and_repeat_the_eager_call(dev, qt, kt):
+    """Append, decode and a packed prefill captured on a caller stream with the caller's workspaces:
+    replays with eager work between them, the integer arrays changed under the graph."""
+    from test_gpu_runtime import _hip
+    hip, lib = _hip(), _lib.load()
+    hkv, G, D, ps, lens = 2, 4, 128, 16, [700, 33, 1]
+    s = Setup(dev, 29, lens, ps, hkv, D, kt, junk=0.5)
+    s.upload()
+    q, qp = s.rng.standard_normal((3, hkv * G, D)).astype(qt), s.rng.standard_normal((40, hkv * G, D)).astype(qt)
+    tq, tp, to, tpo = put(dev, q), put(dev, qp), put(dev, np.zeros_like(q)), put(dev, np.zeros_like(qp))
+    cu1, cu2 = put(dev, np.arange(4, dtype=np.int32)), put(dev, np.asarray([0, 30, 40, 40], np.int32))
+    rows = put(dev, s.rng.standard_normal((3, 2, hkv * D)).astype(NP[kt]))
+    need = max(lib.tl_hip_paged_attention_workspace(3, n, hkv * G, hkv, D) for n in (3, 40))
+    ws = dev.tensor_zeros((need // 4,), F32)
+    dev.synchronize()
+    cache = (s.tk.data_ptr, s.tv.data_ptr, kt, s.n_pages, ps)
+    qd = F16 if qt == np.float16 else F32
+    row, head = hkv * D, hkv * G * D
+    es = 2 if kt == F16 else 4
+
+    def step(stream):
+        rc = lib.tl_hip_launch_kv_append(rows.data_ptr, rows.data_ptr + row * es, kt, 2 * row, 2 * row, *cache, hkv, D,
+                                         s.tt.data_ptr, s.width, cu1.data_ptr, s.tl.data_ptr, 3, 3, stream)
+        rc = rc or lib.tl_hip_launch_paged_attention_decode(tq.data_ptr, qd, head, *cache, hkv * G, hkv, D, s.tt.data_ptr, s.width,
+                                                            s.tl.data_ptr, 3, to.data_ptr, 0.09, ws.data_ptr, need, stream)
+        rc = rc or lib.tl_hip_launch_paged_attention_prefill(tp.data_ptr, qd, head, *cache, hkv * G, hkv, D, s.tt.data_ptr, s.width,
+                                                             cu2.data_ptr, s.tl.data_ptr, 3, 40, tpo.data_ptr, 0.09, ws.data_ptr,
+                                                             need, stream)
+        assert rc == 0, lib.tl_hip_last_error()
+
+    st, graph, run = _stream(hip), C.c_void_p(), C.c_void_p()
+    try:
+        step(st)   # the first call on a stream is not captured
+        assert hip.hipStreamSynchronize(st) == 0
+        assert hip.hipStreamBeginCapture(st, 2) == 0   # relaxed
+        step(st)
+        # without the caller's workspace a captured call is refused
+        assert lib.tl_hip_launch_paged_attention_decode(tq.data_ptr, qd, head, *cache, hkv * G, hkv, D, s.tt.data_ptr, s.width,
+                                                        s.tl.data_ptr, 3, to.data_ptr, 0.09, None, 0, st) == 8
+        assert hip.hipStreamEndCapture(st, C.byref(graph)) == 0
+        assert hip.hipGraphInstantiate(C.byref(run), graph, None, None, 0) == 0
+        for lens in ([700, 33, 1], [650, 1, 0], [16, 30, 1], [700, 33, 1]):
+            new = np.asarray(lens, np.int32)
+            assert lib.tl_hip_memcpy_h2d(s.tl.data_ptr, new.ctypes.data, new.nbytes) == 0
+            step(None)
+            want = get(to, qt, q.shape), get(tpo, qt, qp.shape)
+            for t, a in ((to, q), (tpo, qp)):
+                z = np.zeros_like(a)
+                assert lib.tl_hip_memcpy_h2d(t.data_ptr, z.ctypes.data, z.nbytes) == 0
+            assert hip.hipGraphLaunch(run, st) == 0
+            assert hip.hipStreamSynchronize(st) == 0
+            assert np.array_equal(get(to, qt, q.shape), want[0])
+            assert np.array_equal(get(tpo, qt, qp.shape), want[1])
+    finally:
+        hip.hipStreamSynchronize(st)
+        if run:
+            hip.hipGraphExecDestroy(run)
+        if graph:
+            hip.hipGraphDestroy(graph)
+        hip.hipStreamDestroy(st)
+
+
+def test_calls_that_overlap_on_two_streams(dev):
+    """Two streams at once, each its own sequences, one with the library's workspaces and one with its
+    own: every result is the one alone."""
+    from test_gpu_runtime import _hip
+    hip, lib = _hip(), _lib.load()
+    st = [_stream(hip) for _ in range(2)]
+    try:
+        sets = []
+        for i, lens in enumerate(([9000, 100], [40, 6000, 7])):
+            s = Setup(dev, 30 + i, lens, 64, 2, 128, F16)
+            q = s.rng.standard_normal((len(lens), 16, 128)).astype(np.float32)
+            want = run_attention(s, q, 0.09)
+            check(want, *attention(q, s.k, s.v, s.table, lens, range(len(lens) + 1), 64, 0.09, False))
+            need = lib.tl_hip_paged_attention_workspace(len(lens), len(lens), 16, 2, 128)
+            ws = dev.tensor_zeros((need // 4,), F32) if i else None
+            sets.append((s, put(dev, q), [put(dev, np.zeros_like(q)) for _ in range(8)], ws, need, want))
+        dev.synchronize()
+        for k in range(8):
+            for (s, tq, outs, ws, need, _), stream in zip(sets, st):
+                rc = lib.tl_hip_launch_paged_attention_decode(
+                    tq.data_ptr, F32, 16 * 128, s.tk.data_ptr, s.tv.data_ptr, F16, s.n_pages, 64, 16, 2, 128, s.tt.data_ptr, s.width,
+                    s.tl.data_ptr, len(s.lens), outs[k].data_ptr, 0.09, ws.data_ptr if ws else None, need if ws else 0, stream)
+                assert rc == 0, lib.tl_hip_last_error()
+        for stream in st:
+            assert hip.hipStreamSynchronize(stream) == 0
+        for s, tq, outs, ws, need, want in sets:
+            for o in outs:
+                assert np.array_equal(get(o, np.float32, want.shape), want)
+    finally:
+        for stream in st:
+            hip.hipStreamSynchronize(stream)
+            hip.hipStreamDestroy(stream)
+
+
 # ------------------------------------------------------------------- append, copy ----
 @pytest.mark.parametrize("nt,kt", [(F32, F16), (F32, F32), (F16, F16), (F16, F32)])
 @pytest.mark.parametrize("hkv,D,ps,new,past,extra", [
@@ -391,7 +538,7 @@ def test_append(dev, nt, kt, hkv, D, ps, new, past, extra):
     s = Setup(dev, 21, lens, ps, hkv, D, kt, junk=3.0)
     cu = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
     rows = s.rng.standard_normal((cu[-1] + extra, 2 * hkv * D + 16)).astype(NP[nt])
-    if rows.size > 40:
+    with np.errstate(over="ignore"):
         rows[0, :4] = [65520.0, -1e-8, np.inf, 6e-5]   # past f16's range, below its steps, infinite, subnormal
     s.upload()
     tr, tc = put(dev, rows), put(dev, cu)
@@ -400,7 +547,7 @@ def test_append(dev, nt, kt, hkv, D, ps, new, past, extra):
                                      s.tv.data_ptr, kt, s.n_pages, ps, hkv, D, s.tt.data_ptr, s.width, tc.data_ptr,
                                      s.tl.data_ptr, len(lens), rows.shape[0], None)
     assert rc == 0, lib.tl_hip_last_error()
-    with np.errstate(over="ignore"):
+    with np.errstate(over="ignore"):   # (65520 rounds to infinity)
         for i, (t, want) in enumerate(((s.tk, s.k.copy()), (s.tv, s.v.copy()))):
             for b, n in enumerate(lens):
                 j = np.arange(past[b], n)
