@@ -222,12 +222,17 @@ int tl_hip_debug_last_gemm_plan(int* tile_m, int* tile_n, int* k_splits);
  * The integer arrays are device memory and read by the kernels (a captured call follows their
  * current values at each replay); what they may hold is checked there, never followed out of
  * range: values of cu_seqlens outside 0 .. n_tokens and kv_lens outside 0 .. table_stride *
- * page_size are taken as the nearest bound, and a row belongs to the first sequence that claims it.  A table entry outside 0 .. n_pages - 1 makes the
- * attention rows that see its positions NaN, and appends nothing; so does a kv_lens past the
- * table's positions for the rows at positions past them.  Entries past a sequence's length are
- * not read.
- * Pointers to keys, values, queries and rows are 16-byte aligned, and row strides (in elements)
- * multiples of 16 bytes (ArgumentError otherwise).  stream NULL = the library's.  Sequences are
+ * page_size are taken as the nearest bound, and a row belongs to the first sequence that claims
+ * it.  A table entry outside 0 .. n_pages - 1 makes the attention rows that see its positions NaN,
+ * and appends nothing; so does a kv_lens past the table's positions for the rows at positions past
+ * them.  Entries past a sequence's length are not read.
+ * Limits (ArgumentError past them): n_kv_heads 1024, n_heads 4096 and a multiple of n_kv_heads,
+ * batch 65536, n_tokens 2^24, n_tokens * n_heads 2^26, batch * n_kv_heads 2^22, table_stride *
+ * page_size 2^30; and about 2^31 rounds of 64 to 256 positions that attention could take over all
+ * sequences, heads and groups of 16 rows if every table were full.
+ * Pointers to keys, values, queries and rows are 16-byte aligned, integer arrays 4-byte aligned,
+ * and row strides (in elements) multiples of 16 bytes (ArgumentError otherwise).  stream NULL =
+ * the library's.  Sequences are
  * independent: two calls overlap on different streams as long as neither writes what the other
  * reads.
  *

@@ -4,7 +4,7 @@ import ctypes as C
 
 import pytest
 
-from tl_amd import _lib
+from tl_amd import BackendError, PagedKV, _lib
 
 F32, F16 = 0, 1
 P = 1 << 20  # an aligned address that no refused call follows
@@ -94,3 +94,56 @@ def test_workspace_sizes():
     assert ws(32, 32, 32, 8, 128) > 0 and ws(1, 8192, 32, 8, 256) > 0
     for bad in ((-1, 1, 32, 8, 128), (1, 1, 30, 8, 128), (1, 1, 32, 8, 100), (1, 1 << 25, 32, 8, 128)):
         assert ws(*bad) == 0 and _lib.load().tl_hip_last_status() == 8
+
+
+@pytest.mark.parametrize("name", ["table", "cu", "lens"])
+def test_integer_arrays_off_their_alignment(name):
+    _refused(_append(**{name: P + 2}), 8)
+    _refused(_attend(False, **{name: P + 2}), 8)
+    if name != "cu":
+        _refused(_attend(True, **{name: P + 2}), 8)
+
+
+class _NoDevice:
+    """What PagedKV asks of a device, without one: its launches end in an error."""
+
+    class Tensor:
+        def __init__(self, shape, dtype):
+            self.shape, self.dtype, self.data_ptr = tuple(shape), dtype, P
+
+    def __init__(self):
+        self.lib = _lib.load()
+
+    def tensor_zeros(self, shape, dtype=F32):
+        return self.Tensor(shape, dtype)
+
+    def tensor_new(self, a):
+        return self.Tensor(a.shape, F32)
+
+
+def _kv():
+    kv = PagedKV(_NoDevice(), 8, 16, 2, 64)
+    return kv, kv.open(), kv.open()
+
+
+@pytest.mark.parametrize("counts", [[1], [1, 1, 1], [3, -1]])
+def test_prefill_wants_a_row_count_per_sequence(counts):
+    kv, a, b = _kv()
+    with pytest.raises(BackendError):
+        kv.prefill([a, b], counts, _NoDevice.Tensor((sum(counts), 4, 64), F32), 0.1)
+
+
+def test_an_append_that_fails_leaves_the_lengths():
+    kv, a, b = _kv()
+    kv.book.grow(a, 5)
+    rows = _NoDevice.Tensor((16 * 8, 2, 64), F32)
+    with pytest.raises(BackendError):   # a's 100 fit, b's 28 do not
+        kv.append([a, b], [100, 28], rows, rows)
+    assert (kv.length(a), kv.length(b), kv.book.free_pages) == (5, 0, 7)
+    rows = _NoDevice.Tensor((9, 2, 64), 5)   # a type that the launcher refuses
+    with pytest.raises(BackendError):
+        kv.append([a, b], [4, 5], rows, rows)
+    assert (kv.length(a), kv.length(b), kv.book.free_pages) == (5, 0, 7)
+    with pytest.raises(BackendError):
+        kv.append([a, a], [4, 5], rows, rows)
+    assert kv.length(a) == 5

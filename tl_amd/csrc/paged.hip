@@ -93,6 +93,12 @@ static int arg_error(const char* what) {
     return TL_HIP_ERR_ARG;
 }
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+// (null is aligned: decode has no cu_seqlens)
+static int check_ints(const void* table, const void* cu, const void* lens) {
+    for (const void* p : {table, cu, lens})
+        if (reinterpret_cast<uintptr_t>(p) & 3) return arg_error("page_table, cu_seqlens and kv_lens must be 4-byte aligned");
+    return TL_HIP_OK;
+}
 
 // Sizes that every entry shares; fills c.
 static int check_cache(PagedCache* c, int kv_dtype, int64_t n_pages, int page_size, int hkv, int D, int64_t table_stride,
@@ -195,6 +201,7 @@ static int check_attention(PagedAttn* a, const void* q, int q_dtype, int64_t q_s
     if (rows * hq > (1 << 26) || batch * hkv > (1 << 22)) return arg_error("n_tokens * n_heads must be at most 2^26, batch * n_kv_heads 2^22");
     const int per16 = q_dtype == TL_HIP_F16 ? 8 : 4;
     if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out)) return arg_error("q, pages and out must be 16-byte aligned");
+    if (int rc = check_ints(table, cu, lens)) return rc;
     if (q_stride % per16 || q_stride < (int64_t)hq * D || q_stride > (int64_t(1) << 40))
         return arg_error("q_row_stride must be a multiple of 16 bytes and hold n_heads * head_dim elements");
     if (!std::isfinite(scale)) return arg_error("scale must be finite");
@@ -227,6 +234,7 @@ int tl_hip_launch_kv_append(const void* k_new, const void* v_new, int new_dtype,
     }
     const int64_t width = (int64_t)n_kv_heads * head_dim, per16 = new_dtype == TL_HIP_F16 ? 8 : 4;
     if (!aligned16(k_new) || !aligned16(v_new) || !aligned16(k_pages) || !aligned16(v_pages)) return arg_error("rows and pages must be 16-byte aligned");
+    if (int rc = check_ints(page_table, cu_seqlens, kv_lens)) return rc;
     for (int64_t st : {k_row_stride, v_row_stride})
         if (st % per16 || st < width || st > (int64_t(1) << 40))
             return arg_error("row strides must be multiples of 16 bytes and hold n_kv_heads * head_dim elements");

@@ -596,7 +596,8 @@ __global__ __launch_bounds__(64 * NW, (DP > 128 ? 1 : 2)) void k_paged_tile(
 
 // ---- prompts: which work is whose ----
 // Tiles of 2^shift rows, `unit` = KV head + n_kv_heads * tile: heads next to each other (on XCDs
-// of their own), tiles from the last one back, so that of one sequence the longest come first.
+// of their own), the tiles that see most first (beyond 64 sequences: of each sequence).  Seven
+// prompts, 4001 rows together, 1024 units: 77 us, against 82 with the sequences one by one.
 // A call with few units cuts each unit's positions into SLOTS / units parts, of about four K/V
 // tiles at least; a workgroup takes unit blockIdx % units, part blockIdx / units, and leaves a
 // record (o, m, l, c of its rows) in slot unit * (SLOTS / units) + part, which k_prompt_join adds.
@@ -623,19 +624,45 @@ __device__ __forceinline__ bool prompt_tile(const PagedCache& c, const int32_t* 
     p->unit = cut && !whole_units ? index % p->units : index;
     if (p->unit >= p->units) return false;
     p->h = p->unit % c.hkv;
-    const int nth = total - 1 - p->unit / c.hkv;
+    // tiles before this one; the second 256 units, which share CUs with the first, come shortest first
+    int nth = p->unit / c.hkv;
+    const int one = 256 / c.hkv, two = min(2 * one, total);
+    if (nth >= one && nth < two) nth = one + two - 1 - nth;
+    if (c.batch <= 64) {
+        // Longest first: tile t of a sequence weighs first + t, its position in tiles.  The nth
+        // heaviest of all weighs the most that more than nth tiles weigh or pass.
+        const int first = (int)max(min(((int64_t)grp.q.shown * G) >> shift, (int64_t)1 << 29), -((int64_t)1 << 29));
+        auto reach = [&](int w) {  // tiles that weigh w or more
+            return lane_value(lane_prefix(max(min(first + mine - w, mine), 0)), 63);
+        };
+        int lo = mine > 0 ? first : 1 << 30, hi = mine > 0 ? first + mine - 1 : -(1 << 30);  // (total is not 0)
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) lo = min(lo, __shfl_xor(lo, off)), hi = max(hi, __shfl_xor(hi, off));
+        lo = __builtin_amdgcn_readfirstlane(lo), hi = __builtin_amdgcn_readfirstlane(hi);
+        while (lo < hi) {
+            const int mid = lo + ((hi - lo + 1) >> 1);
+            if (reach(mid) > nth) lo = mid;
+            else hi = mid - 1;
+        }
+        int skip = nth - reach(lo + 1);
+        uint64_t hit = __ballot(lo >= first && lo - first < mine);
+        for (; skip > 0; skip--) hit &= hit - 1;
+        p->b = __builtin_ctzll(hit);
+        p->tile = lo - lane_value(first, p->b);
+        p->sq = grp.at(p->b);
+        return true;
+    }
     int before = 0;
     for (int base = 0;; base += 64) {
-        if (c.batch > 64) {
-            grp.load(c, cu, lens, base);
-            mine = (grp.q.n * G + up) >> shift;
-            incl = lane_prefix(mine);
-        }
+        grp.load(c, cu, lens, base);
+        mine = (grp.q.n * G + up) >> shift;
+        incl = lane_prefix(mine);
         const uint64_t hit = __ballot(nth < before + incl);
         if (hit) {
             const int at = __builtin_ctzll(hit);
             p->b = base + at;
-            p->tile = __builtin_amdgcn_readfirstlane((nth - (before + lane_value(incl, at) - lane_value(mine, at))));
+            const int t = nth - (before + lane_value(incl, at) - lane_value(mine, at));
+            p->tile = lane_value(mine, at) - 1 - t;
             break;
         }
         before += lane_value(incl, 63);

@@ -139,10 +139,10 @@ class PagedKV:
                 dst.ctypes.data_as(_lib.i32p), len(pairs), self.lib.tl_hip_stream()))
 
     def _tables(self, seqs, counts):
-        """The tensor that holds them, and device addresses of the page table, cu_seqlens and kv_lens of these sequences, and the
-        table's width."""
-        if len(set(seqs)) != len(seqs):
-            raise BackendError(8, "ArgumentError: a sequence appears once per call")
+        """The tensor that holds them, device addresses of the page table, cu_seqlens and kv_lens of
+        these sequences, and the table's width."""
+        if len(set(seqs)) != len(seqs) or len(counts) != len(seqs) or min([0, *counts]) < 0:
+            raise BackendError(8, "ArgumentError: a sequence appears once per call, with its number of rows")
         lens = [self.book.length(s) for s in seqs]
         width = max([1] + [-(-n // self.book.page_size) for n in lens])
         rows = [self.book.row(s, width) for s in seqs]
@@ -161,20 +161,22 @@ class PagedKV:
             raise BackendError(7, "TypeMismatch: k and v of one dtype")
         if len(set(seqs)) != len(seqs):
             raise BackendError(8, "ArgumentError: a sequence appears once per call")
-        before = [self.book.length(s) for s in seqs]
-        for i, (s, n) in enumerate(zip(seqs, counts)):
-            try:
-                self._copy(self.book.grow(s, n))
-            except Exception:
-                for t, was in zip(seqs[:i], before):
-                    self.book.cut(t, was)
-                raise
-        held, table, cu, lens, width = self._tables(seqs, counts)
-        row = self.n_kv_heads * self.head_dim
-        self._check(self.lib.tl_hip_launch_kv_append(
-            k.data_ptr, v.data_ptr, k.dtype, row, row, self.k.data_ptr, self.v.data_ptr, self.dtype, self.book.n_pages,
-            self.book.page_size, self.n_kv_heads, self.head_dim, table, width, cu, lens, len(seqs), total,
-            self.lib.tl_hip_stream()))
+        before, grown = [self.book.length(s) for s in seqs], 0
+        try:
+            for s, n in zip(seqs, counts):
+                pairs = self.book.grow(s, n)
+                grown += 1
+                self._copy(pairs)
+            held, table, cu, lens, width = self._tables(seqs, counts)
+            row = self.n_kv_heads * self.head_dim
+            self._check(self.lib.tl_hip_launch_kv_append(
+                k.data_ptr, v.data_ptr, k.dtype, row, row, self.k.data_ptr, self.v.data_ptr, self.dtype, self.book.n_pages,
+                self.book.page_size, self.n_kv_heads, self.head_dim, table, width, cu, lens, len(seqs), total,
+                self.lib.tl_hip_stream()))
+        except Exception:
+            for s, was in zip(seqs[:grown], before):
+                self.book.cut(s, was)
+            raise
 
     def _rows(self, q, total):
         if len(q.shape) != 3 or q.shape[0] != total or q.shape[2] != self.head_dim:
@@ -183,6 +185,7 @@ class PagedKV:
 
     def decode(self, seqs, q, scale):
         """q [len(seqs), n_heads, head_dim], the newest position of each -> the same shape."""
+        seqs = list(seqs)
         heads, out = self._rows(q, len(seqs))
         held, table, _, lens, width = self._tables(seqs, [1] * len(seqs))
         self._check(self.lib.tl_hip_launch_paged_attention_decode(
@@ -193,7 +196,7 @@ class PagedKV:
 
     def prefill(self, seqs, counts, q, scale):
         """q [sum(counts), n_heads, head_dim]: the last counts[i] positions of seqs[i], causal."""
-        total = int(sum(counts))
+        total, seqs = int(sum(counts)), list(seqs)
         heads, out = self._rows(q, total)
         held, table, cu, lens, width = self._tables(seqs, counts)
         self._check(self.lib.tl_hip_launch_paged_attention_prefill(
