@@ -190,6 +190,54 @@ def test_prefill_of_long_prompts(dev, qt, kt, hkv, G, D, ps, new, past, extra, r
 
 
 @pytest.mark.parametrize("qt,kt", TYPES)
+@pytest.mark.parametrize("hkv,G,D,room", [(64, 2, 64, 0), (1, 3, 64, 65536), (1, 2, 128, 65536)])
+def test_prefill_of_many_short_prompts(dev, qt, kt, hkv, G, D, room):
+    """More sequences than lanes, empty ones and ones with more rows than positions among them."""
+    r = np.random.default_rng(33)
+    new = r.integers(0, 30, 83)
+    lens = [int(n + p) for n, p in zip(new, r.integers(-4, 40, 83))]
+    lens = [max(n, 0) for n in lens]
+    s = Setup(dev, 34, lens, 16, hkv, D, kt, width=room // 16 or None)
+    cu = np.concatenate([[0], np.cumsum(new)])
+    q = s.rng.standard_normal((cu[-1] + 1, hkv * G, D)).astype(qt)
+    check(run_attention(s, q, 0.2, cu=cu), *attention(q, s.k, s.v, s.table, lens, cu, 16, 0.2, qt == np.float16))
+
+
+@pytest.mark.parametrize("qt,kt", TYPES)
+@pytest.mark.parametrize("hkv,room", [(2, 16384), (64, 512)])   # positions cut, and whole
+def test_prompts_over_bad_pages_lengths_and_offsets(dev, qt, kt, hkv, room):
+    new, past, G, D = [170, 40], [90, 0], 4, 64
+    lens = [n + p for n, p in zip(new, past)]
+    s = Setup(dev, 35, lens, 16, hkv, D, kt, width=room // 16)
+    cu = np.concatenate([[0], np.cumsum(new)])
+    q = s.rng.standard_normal((210, hkv * G, D)).astype(qt)
+    want = run_attention(s, q, 0.2, cu=cu)
+    check(want, *attention(q, s.k, s.v, s.table, lens, cu, 16, 0.2, qt == np.float16))
+    good = s.table.copy()
+    for entry in (-1, 1 << 30, -(1 << 31)):
+        s.table[0, 9] = entry   # positions 144 .. 159
+        got = run_attention(s, q, 0.2, cu=cu)
+        first = 144 - past[0]
+        assert np.isnan(got[first:170]).all()
+        assert np.array_equal(got[:first], want[:first]) and np.array_equal(got[170:], want[170:])
+    s.table = good
+    # a length past the table: rows at positions past its end are NaN, those before see what it holds
+    s.width = 16
+    s.table = np.ascontiguousarray(good[:, :16])
+    s.lens = [260, 40]
+    if hkv == 64:
+        got = run_attention(s, q, 0.2, cu=cu)
+        assert np.isnan(got[166:170]).all() and np.isfinite(got[:166]).all() and np.array_equal(got[170:], want[170:])
+        assert np.array_equal(got[:166], want[:166])
+    s.table, s.width = good, room // 16
+    # offsets that fall or leave the rows: the first to claim a row has it
+    got = run_attention(s, q, 0.2, cu=[0, 170, 1 << 30])
+    assert np.array_equal(got, want)
+    got = run_attention(s, q, 0.2, cu=[-5, 170, 90])
+    assert np.array_equal(got[:170], want[:170]) and np.all(got[170:] == 7)
+
+
+@pytest.mark.parametrize("qt,kt", TYPES)
 @pytest.mark.parametrize("hkv,G,D", [(2, 5, 64), (1, 8, 40), (1, 4, 80), (2, 16, 128)])
 def test_decode_of_few_long_sequences(dev, qt, kt, hkv, G, D):
     lens = [5000, 0, 1, 4097]
@@ -480,6 +528,67 @@ def test_graphs_follow_the_lengths_and_repeat_the_eager_call(dev, qt, kt):
             assert hip.hipStreamSynchronize(st) == 0
             assert np.array_equal(get(to, qt, q.shape), want[0])
             assert np.array_equal(get(tpo, qt, qp.shape), want[1])
+    finally:
+        hip.hipStreamSynchronize(st)
+        if run:
+            hip.hipGraphExecDestroy(run)
+        if graph:
+            hip.hipGraphDestroy(graph)
+        hip.hipStreamDestroy(st)
+
+
+@pytest.mark.parametrize("qt,kt", TYPES)
+def test_captured_prompts_and_page_copies(dev, qt, kt):
+    """A fork's page copies and a prompt whose positions are cut, in one graph: the pairs are the
+    graph's own, the rows follow the pages."""
+    from test_gpu_runtime import _hip
+    hip, lib = _hip(), _lib.load()
+    hkv, G, D, ps = 2, 4, 128, 64
+    s = Setup(dev, 36, [400, 130], ps, hkv, D, kt, width=512, junk=0.25)
+    s.upload()
+    cu = np.asarray([0, 200, 330], np.int32)
+    q = s.rng.standard_normal((330, hkv * G, D)).astype(qt)
+    tq, tc, to = put(dev, q), put(dev, cu), put(dev, np.zeros_like(q))
+    need = lib.tl_hip_paged_attention_workspace(2, 330, hkv * G, hkv, D)
+    ws = dev.tensor_zeros((need // 4,), F32)
+    es = 2 if kt == F16 else 4
+    spare = [p for p in range(s.n_pages) if p not in s.table]
+    src, dst = np.asarray([s.table[0, 0]], np.int32), np.asarray(spare[:1], np.int32)   # sequence 0's first page to a spare one
+    s.table[0, 0] = spare[0]
+    assert lib.tl_hip_synchronize() == 0
+    assert lib.tl_hip_memcpy_h2d(s.tt.data_ptr, s.table.ctypes.data, s.table.nbytes) == 0
+
+    def step(stream):
+        rc = lib.tl_hip_launch_kv_copy_pages(s.tk.data_ptr, s.tv.data_ptr, 1, s.n_pages, hkv * ps * D * es,
+                                             src.ctypes.data_as(_lib.i32p), dst.ctypes.data_as(_lib.i32p), 1, stream)
+        rc = rc or lib.tl_hip_launch_paged_attention_prefill(
+            tq.data_ptr, F16 if qt == np.float16 else F32, hkv * G * D, s.tk.data_ptr, s.tv.data_ptr, kt, s.n_pages, ps, hkv * G,
+            hkv, D, s.tt.data_ptr, s.width, tc.data_ptr, s.tl.data_ptr, 2, 330, to.data_ptr, 0.09, ws.data_ptr, need, stream)
+        assert rc == 0, lib.tl_hip_last_error()
+
+    k = s.k.copy()
+    for x in (s.k, s.v):
+        x[spare[0]] = x[src[0]]
+    st, graph, run = _stream(hip), C.c_void_p(), C.c_void_p()
+    try:
+        step(st)
+        assert hip.hipStreamSynchronize(st) == 0
+        assert hip.hipStreamBeginCapture(st, 2) == 0
+        step(st)
+        assert hip.hipStreamEndCapture(st, C.byref(graph)) == 0
+        src[0], dst[0] = dst[0], src[0]   # the graph has its pairs
+        assert hip.hipGraphInstantiate(C.byref(run), graph, None, None, 0) == 0
+        for lens in ([400, 130], [300, 100], [400, 130]):
+            new = np.asarray(lens, np.int32)
+            assert lib.tl_hip_memcpy_h2d(s.tl.data_ptr, new.ctypes.data, new.nbytes) == 0
+            junk = np.full(k[0].shape, 9, NP[kt])
+            at = int(spare[0]) * junk.nbytes
+            assert lib.tl_hip_memcpy_h2d(s.tk.data_ptr + at, junk.ctypes.data, junk.nbytes) == 0
+            z = np.full_like(q, 7)
+            assert lib.tl_hip_memcpy_h2d(to.data_ptr, z.ctypes.data, z.nbytes) == 0
+            assert hip.hipGraphLaunch(run, st) == 0
+            assert hip.hipStreamSynchronize(st) == 0
+            check(get(to, qt, q.shape), *attention(q, s.k, s.v, s.table, lens, cu, ps, 0.09, qt == np.float16))
     finally:
         hip.hipStreamSynchronize(st)
         if run:
