@@ -15,7 +15,7 @@ namespace tlhip {
 // Every new row is read once and written once: HBM bound.  A workgroup takes TOKENS rows, a thread
 // the same 8 elements of each (16-byte stores, the loads of all rows requested first); its
 // wavefronts find the rows' places for themselves, a lane per sequence.  8192 f32 rows of 8 heads of
-// 128 into f16 pages (101 MB): 20.8 us, 4.8 TB/s, with 1 to 4 rows per workgroup alike.
+// 128 into f16 pages (101 MB): 20.4 us, 4.9 TB/s, with 1 to 4 rows per workgroup alike.
 struct AppendArgs {
     PagedCache c;
     const void* kn;
@@ -69,7 +69,7 @@ __global__ __launch_bounds__(256) void k_kv_append(const AppendArgs a, const int
 // ---- page copies ---------------------------------------------------------------------
 // Bytes read and written once: HBM bound.  The pairs travel in the kernel's arguments (at most
 // 4 KiB): nothing to upload, and a captured call keeps its own.  16 bytes per thread, past the
-// caches: 768 pages of 128 KiB, K and V (403 MB) 68.8 us, 5.9 TB/s (74.9 us through the caches;
+// caches: 768 pages of 128 KiB, K and V (403 MB) 68.4 us, 5.9 TB/s (74.9 us through the caches;
 // 79.8 with four loads per thread).
 constexpr int COPY_PAIRS = 440;
 struct CopyArgs {

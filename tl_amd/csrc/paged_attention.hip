@@ -66,8 +66,9 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
 }
 
 // Adds the parts of a tile's records, in order, and writes its rows: part 0 at byte `first` of the
-// workspace, part i at rest + i step.  A thread per four elements, over all parts or, where the rows are few, over every `slices`-th
-// and then over the slices.  Eight parts are requested at a time.
+// workspace, part i at rest + i step.  A thread per four elements, over all parts or, where the rows
+// are few, over every `slices`-th and then over the slices.  Eight parts are requested at a time (one
+// by one, 64 parts took 44 us).
 constexpr int JOIN_ROOM = 7;  // floats of LDS per thread
 template <typename QT, int POLICY, int NT>  // NT threads
 __device__ __forceinline__ void join_tile(const PagedAttn& a, const Seq& sq, int h, int tile, uint32_t first, uint32_t rest,
@@ -158,6 +159,9 @@ __device__ uint32_t g_paged_arrive[RUNS];
 // f16 caches: products exact in f32; f32 rows enter as two f16 parts (row scaled by a power of
 // two, 22 bits), weights as two parts of 2^15 p, so the results keep f32's digits.  f32 caches:
 // f32 matrix instructions.
+// Long caches are bound by HBM: 32 ragged sequences of up to 8192, 8 KV heads of 128 (543 MB) 91 us,
+// 5.9 TB/s; 2 of up to 131072 126 us, 6.5 TB/s.  Short ones by the launch, the reads of lengths,
+// table and keys, each waiting for the one before, and the join: one sequence of 512 7.6 us.
 template <typename KVT, typename QT, int DP, int TK, int NW>
 struct Tile {
     static constexpr bool H16 = std::is_same_v<KVT, _Float16>;
@@ -686,7 +690,11 @@ __device__ __forceinline__ int prompt_parts(int most, int tiles) { return max(mi
 // positions past the last one seen and of dimensions past head_dim, lie outside the buffer
 // resources and arrive as zeros.
 // 16-byte chunks of K rows are spread by the row, so that 16 rows of one chunk lie in 16
-// different places of the banks; chunks of V rows by quarters, for four rows of 64 bytes.
+// different places of the banks; chunks of V rows by quarters, for four rows of 64 bytes (no bank
+// conflicts counted).
+// Bound by the matrix units, at the card's power limit in long calls: 8192 rows over 8192 positions
+// and themselves, 32 heads over 8 of 128, f16 rows 1.65 ms, 1000 TFLOP/s; f32 rows take every
+// product twice, 7 prompts of 4001 rows together 72 us.
 template <int DP>
 struct PromptTile {
     static constexpr int KT = DP > 128 ? 32 : 64;
@@ -951,7 +959,8 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_prompt(
 // The same with f32 matrix instructions (v_mfma_f32_16x16x4_f32): 64 rows to a workgroup, 16 to a
 // wavefront, 16 KiB of keys and of values at a time.  Lane (col, g) holds row col's scores at
 // keys 4 g + e of 16; one 16-byte read of a value row feeds four matrix instructions, dimension
-// 64 j + 4 r + y in row r of number y.
+// 64 j + 4 r + y in row r of number y.  3 prompts of 1100 rows together, 32 heads over 4 of 64: 38 us
+// (2.5 GFLOP, 66 TFLOP/s); while a CU works its matrix units do 59 % of the time.
 template <int DP>
 __global__ __launch_bounds__(256, 2) void k_paged_prompt_f32(
     const PagedAttn a, const int32_t* __restrict__ table, const int32_t* __restrict__ cu, const int32_t* __restrict__ lens,
@@ -1143,7 +1152,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_prompt_f32(
         }
 }
 
-// Adds the parts of cut units, 16 rows to a workgroup.
+// Adds the parts of cut units, 16 rows to a workgroup: a launch, and one wait per eight parts.
 template <typename QT>
 __global__ __launch_bounds__(256) void k_prompt_join(const PagedAttn a, const int32_t* __restrict__ cu, const int32_t* __restrict__ lens, int shift, int keys) {
     __shared__ __attribute__((aligned(16))) float room[256 * JOIN_ROOM];
@@ -1161,7 +1170,8 @@ __global__ __launch_bounds__(256) void k_prompt_join(const PagedAttn a, const in
 }
 
 // The join, one workgroup per (sequence, KV head, tile) that there can be, in the line's order:
-// for calls whose parts are not joined where they were made.
+// for calls whose parts are not joined where they were made (one sequence of 512: the two launches
+// 10.4 us, the one 8.0).
 template <typename QT, bool PACKED, int NT>
 __global__ __launch_bounds__(NT) void k_paged_join(const PagedAttn a, const int32_t* __restrict__ cu, const int32_t* __restrict__ lens, int keys, int runs) {
     __shared__ __attribute__((aligned(16))) float room[NT * JOIN_ROOM];
