@@ -232,9 +232,8 @@ int tl_hip_debug_last_gemm_plan(int* tile_m, int* tile_n, int* k_splits);
  * sequences, heads and groups of 16 rows if every table were full.
  * Pointers to keys, values, queries and rows are 16-byte aligned, integer arrays 4-byte aligned,
  * and row strides (in elements) multiples of 16 bytes (ArgumentError otherwise).  stream NULL =
- * the library's.  Sequences are
- * independent: two calls overlap on different streams as long as neither writes what the other
- * reads.
+ * the library's.  What a call writes overlaps nothing that it reads.  Two calls may run at the same
+ * time on different streams as long as neither writes what the other reads or writes.
  *
  * tl_hip_launch_kv_append writes row t's keys and values (k_new + t * k_row_stride, n_kv_heads *
  * head_dim of new_dtype F32 or F16; likewise v_new) to its position's slot, rounded to nearest
