@@ -8,6 +8,7 @@
 #include "gemm_common.h"
 #include "paged.h"
 
+#include <algorithm>
 #include <cfloat>
 #include <type_traits>
 
@@ -605,17 +606,17 @@ __global__ __launch_bounds__(64 * NW, (DP > 128 ? 1 : 2)) void k_paged_tile(
 // Tiles of 2^shift rows, `unit` = KV head + n_kv_heads * tile: heads next to each other (on XCDs
 // of their own), the tiles that see most first (beyond 64 sequences: of each sequence).  Seven
 // prompts, 4001 rows together, 1024 units: 77 us, against 82 with the sequences one by one.
-// A call with few units cuts each unit's positions into SLOTS / units parts, of about four K/V
-// tiles at least; a workgroup takes unit blockIdx % units, part blockIdx / units, and leaves a
-// record (o, m, l, c of its rows) in slot unit * (SLOTS / units) + part, which k_prompt_join adds.
+// A call with few units cuts each unit's positions into up to `most` parts, of about four K/V
+// tiles at least; a workgroup takes unit index % units, part index / units, and leaves a record
+// (o, m, l, c of its rows) in slot unit * most + part, which k_prompt_join adds.
 constexpr int SLOTS = 512;
 struct Prompt {
     Seq sq;
-    int b, h, tile, unit, units, most;  // most: parts per unit, at most
+    int b, h, tile, unit, units;
 };
-// cut: whether units are cut; index: the workgroup's, or with cut the one of SLOTS.
+// index: the workgroup's or, with whole, a unit's.
 __device__ __forceinline__ bool prompt_tile(const PagedCache& c, const int32_t* cu, const int32_t* lens, int G, int shift, int index,
-                                            bool cut, bool whole_units, Prompt* p) {
+                                            int most, bool whole, Prompt* p) {
     const int up = (1 << shift) - 1;
     Group<true> grp;
     int total = 0, incl = 0, mine = 0;
@@ -627,8 +628,7 @@ __device__ __forceinline__ bool prompt_tile(const PagedCache& c, const int32_t* 
     }
     p->units = total * c.hkv;  // (rows and heads together are below 2^27)
     if (p->units == 0) return false;
-    p->most = cut ? max(SLOTS / p->units, 1) : 1;
-    p->unit = cut && !whole_units ? index % p->units : index;
+    p->unit = most > 1 && !whole ? index % p->units : index;
     if (p->unit >= p->units) return false;
     p->h = p->unit % c.hkv;
     // tiles before this one; the second 256 units, which share CUs with the first, come shortest
@@ -707,10 +707,13 @@ struct PromptTile {
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef short short4v __attribute__((ext_vector_type(4)));
 
-template <typename QT, int DP>
-__global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_prompt(
+// W: groups of four wavefronts.  With two each takes every second tile of the workgroup's, in
+// buffers of its own, and the second's sums reach the first through LDS: for calls whose units are
+// about as many as the CUs.
+template <typename QT, int DP, int W>
+__global__ __launch_bounds__(256 * W, (DP > 128 ? 1 : 2)) void k_paged_prompt(
     const PagedAttn a, const int32_t* __restrict__ table, const int32_t* __restrict__ cu, const int32_t* __restrict__ lens,
-    const char* __restrict__ kp, const char* __restrict__ vp, bool cut) {
+    const char* __restrict__ kp, const char* __restrict__ vp, int most) {
     using L = PromptTile<DP>;
     constexpr int KT = L::KT, CPR = L::CPR, U = L::U, RPW = KT / 4;
     constexpr int QP = std::is_same_v<QT, float> ? 2 : 1;  // f16 parts of a query, and of a weight
@@ -718,13 +721,13 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_prompt(
     struct Stage {
         uint4 k[KT * CPR], v[KT * CPR];
     };
-    __shared__ __attribute__((aligned(16))) Stage S[2];
+    __shared__ __attribute__((aligned(16))) Stage S[2 * W];
     const PagedCache& c = a.c;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, hf = lane >> 5;
+    const int lane = threadIdx.x & 63, wave4 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = wave4 & 3, group = W == 1 ? 0 : wave4 >> 2, col = lane & 31, hf = lane >> 5;
     const int G = a.G, D = c.D, page = 1 << c.shift;
 
     Prompt pt;
-    if (!prompt_tile(c, cu, lens, G, 7, blockIdx.x, cut, false, &pt)) return;
+    if (!prompt_tile(c, cu, lens, G, 7, blockIdx.x, most, false, &pt)) return;
     const Seq sq = pt.sq;
     const int b = pt.b, h = pt.h, tile = pt.tile;
     const int rows = sq.n * G;
@@ -735,9 +738,9 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_prompt(
     const int last = uniform(limit(tile * 128 + 127)), all = uniform(limit(tile * 128));  // positions that any, that every row sees
     const bool live = w0 < rows;
     // this part's K/V tiles
-    const int tiles = (last + KT - 1) / KT, whole = all / KT, parts = prompt_parts(pt.most, tiles), part = blockIdx.x / pt.units;
-    if (cut && part >= parts) return;
-    const int t0 = cut ? (int)((int64_t)tiles * part / parts) : 0, t1 = cut ? (int)((int64_t)tiles * (part + 1) / parts) : tiles;
+    const int tiles = (last + KT - 1) / KT, whole = all / KT, parts = prompt_parts(most, tiles), part = most > 1 ? blockIdx.x / pt.units : 0;
+    if (part >= parts) return;
+    const int t0 = most > 1 ? (int)((int64_t)tiles * part / parts) : 0, t1 = most > 1 ? (int)((int64_t)tiles * (part + 1) / parts) : tiles;
 
     // this lane's part of its row: dimensions 16 s + 8 hf ..
     const QT* qp = static_cast<const QT*>(a.q) + (int64_t)(sq.first + qi) * a.q_stride + qh * D;
@@ -910,32 +913,62 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_prompt(
     };
 
     if (t0 < t1) {
-        int pid = page_of(t0 * KT);
-        issue(t0 * KT, pid, S[t0 & 1]);
-        pid = page_of((t0 + 1) * KT);
-        auto step = [&](int t, auto edge) __attribute__((always_inline)) {
+        auto buffer = [&](int t) { return W == 1 ? t & 1 : 2 * group + (((t - t0) >> 1) & 1); };
+        int pid = page_of((t0 + group) * KT);
+        if (W == 1 || t0 + group < t1) issue((t0 + group) * KT, pid, S[buffer(t0)]);
+        pid = page_of((t0 + W + group) * KT);
+        auto step = [&](int t, auto edge) __attribute__((always_inline)) {  // tiles t .. t + W - 1
             __builtin_amdgcn_s_waitcnt(0xF70);  // vmcnt(0): this tile's DMA has landed
             __syncthreads();
             __builtin_amdgcn_sched_barrier(0);
-            if (t + 1 < t1) {
-                issue((t + 1) * KT, pid, S[(t + 1) & 1]);
-                pid = page_of((t + 2) * KT);
+            const int mine = t + group;
+            if (mine + W < t1) {
+                issue((mine + W) * KT, pid, S[buffer(t + W)]);
+                pid = page_of((mine + 2 * W) * KT);
             }
             __builtin_amdgcn_sched_barrier(0);
-            if (live && t * KT < lim_hi) compute(t * KT, reinterpret_cast<const char*>(&S[t & 1]), edge);
+            if (live && (W == 1 || mine < t1) && mine * KT < lim_hi) compute(mine * KT, reinterpret_cast<const char*>(&S[buffer(t)]), edge);
         };
         int t = t0;
 #pragma unroll 1
-        for (; t < min(whole, t1); t++) step(t, std::false_type{});
+        for (; t + W <= min(whole, t1); t += W) step(t, std::false_type{});
 #pragma unroll 1
-        for (; t < t1; t++) step(t, std::true_type{});
+        for (; t < t1; t += W) step(t, std::true_type{});
     }
     l = lane_pair_sum<32>(l);
+    if constexpr (W == 2) {
+        static_assert(4 * 64 * (16 * DT + 2) * 4 <= (int)sizeof(S), "the second group's sums");
+        floatx4* room = reinterpret_cast<floatx4*>(S) + wave * 64 * 4 * DT;
+        float* ml = reinterpret_cast<float*>(S) + 4 * 64 * 16 * DT + wave * 128 + lane;
+        __syncthreads();  // the tiles are read
+        if (group) {
+#pragma unroll
+            for (int i = 0; i < DT; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    room[(4 * i + e) * 64 + lane] = floatx4{acc[i][4 * e], acc[i][4 * e + 1], acc[i][4 * e + 2], acc[i][4 * e + 3]};
+            ml[0] = m, ml[64] = l;
+        }
+        __syncthreads();
+        if (group) return;
+        const float mo = ml[0], mn = fmaxf(m, mo), ms = mn == -INFINITY ? 0.f : mn;
+        const float f = __builtin_amdgcn_exp2f((m - ms) * cs), fo = __builtin_amdgcn_exp2f((mo - ms) * cs);
+        m = mn;
+        l = fmaf(l, f, ml[64] * fo);
+#pragma unroll
+        for (int i = 0; i < DT; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const floatx4 z = room[(4 * i + e) * 64 + lane];
+#pragma unroll
+                for (int y = 0; y < 4; y++) acc[i][4 * e + y] = fmaf(acc[i][4 * e + y], f, z[y] * fo);
+            }
+    }
     if (w0 + col >= rows) return;
     const int sees = sq.shown + qi;
     const float inv = sees > sq.len ? NAN : 1.0f / l;
     QT* op = static_cast<QT*>(a.out) + ((int64_t)(sq.first + qi) * a.hq + qh) * D;
-    float* rec = a.ws + ((int64_t)(pt.unit * pt.most + part) * 128 + wave * 32 + col) * (D + 4);
+    float* rec = a.ws + ((int64_t)(pt.unit * most + part) * 128 + wave * 32 + col) * (D + 4);
     if (parts > 1 && hf == 0) *reinterpret_cast<floatx4*>(rec + D) = floatx4{m, l, cs, 0.f};
 #pragma unroll
     for (int i = 0; i < DT; i++)
@@ -961,20 +994,20 @@ __global__ __launch_bounds__(256, (DP > 128 ? 1 : 2)) void k_paged_prompt(
 // keys 4 g + e of 16; one 16-byte read of a value row feeds four matrix instructions, dimension
 // 64 j + 4 r + y in row r of number y.  3 prompts of 1100 rows together, 32 heads over 4 of 64: 38 us
 // (2.5 GFLOP, 66 TFLOP/s); while a CU works its matrix units do 59 % of the time.
-template <int DP>
-__global__ __launch_bounds__(256, 2) void k_paged_prompt_f32(
+template <int DP, int W>  // W as above
+__global__ __launch_bounds__(256 * W, 2) void k_paged_prompt_f32(
     const PagedAttn a, const int32_t* __restrict__ table, const int32_t* __restrict__ cu, const int32_t* __restrict__ lens,
-    const char* __restrict__ kp, const char* __restrict__ vp, bool cut) {
+    const char* __restrict__ kp, const char* __restrict__ vp, int most) {
     constexpr int CPR = DP / 4, KT = 1024 / CPR, U = 4, RPW = KT / 4, ST = KT / 16, KS = DP / 16, VN = DP / 64;
     struct Stage {
         uint4 k[KT * CPR], v[KT * CPR];
     };
-    __shared__ __attribute__((aligned(16))) Stage S[2];
+    __shared__ __attribute__((aligned(16))) Stage S[2 * W];
     const PagedCache& c = a.c;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, wave4 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = wave4 & 3, group = W == 1 ? 0 : wave4 >> 2, col = lane & 15, g = lane >> 4;
     const int G = a.G, D = c.D, page = 1 << c.shift;
     Prompt pt;
-    if (!prompt_tile(c, cu, lens, G, 6, blockIdx.x, cut, false, &pt)) return;
+    if (!prompt_tile(c, cu, lens, G, 6, blockIdx.x, most, false, &pt)) return;
     const Seq sq = pt.sq;
     const int b = pt.b, h = pt.h, tile = pt.tile;
     const int rows = sq.n * G;
@@ -985,9 +1018,9 @@ __global__ __launch_bounds__(256, 2) void k_paged_prompt_f32(
     const int last = uniform(limit(tile * 64 + 63)), all = uniform(limit(tile * 64));  // positions that any, that every row sees
     const bool live = w0 < rows;
     // this part's K/V tiles
-    const int tiles = (last + KT - 1) / KT, whole = all / KT, parts = prompt_parts(pt.most, tiles), part = blockIdx.x / pt.units;
-    if (cut && part >= parts) return;
-    const int t0 = cut ? (int)((int64_t)tiles * part / parts) : 0, t1 = cut ? (int)((int64_t)tiles * (part + 1) / parts) : tiles;
+    const int tiles = (last + KT - 1) / KT, whole = all / KT, parts = prompt_parts(most, tiles), part = most > 1 ? blockIdx.x / pt.units : 0;
+    if (part >= parts) return;
+    const int t0 = most > 1 ? (int)((int64_t)tiles * part / parts) : 0, t1 = most > 1 ? (int)((int64_t)tiles * (part + 1) / parts) : tiles;
 
     const float* qp = static_cast<const float*>(a.q) + (int64_t)(sq.first + qi) * a.q_stride + qh * D;
     const float sign = a.scale < 0.f ? -1.f : a.scale > 0.f ? 1.f : 0.f;
@@ -1107,33 +1140,58 @@ __global__ __launch_bounds__(256, 2) void k_paged_prompt_f32(
     };
 
     if (t0 < t1) {
-        int pid = page_of(t0 * KT);
-        issue(t0 * KT, pid, S[t0 & 1]);
-        pid = page_of((t0 + 1) * KT);
-        auto step = [&](int t, auto edge) __attribute__((always_inline)) {
+        auto buffer = [&](int t) { return W == 1 ? t & 1 : 2 * group + (((t - t0) >> 1) & 1); };
+        int pid = page_of((t0 + group) * KT);
+        if (W == 1 || t0 + group < t1) issue((t0 + group) * KT, pid, S[buffer(t0)]);
+        pid = page_of((t0 + W + group) * KT);
+        auto step = [&](int t, auto edge) __attribute__((always_inline)) {  // tiles t .. t + W - 1
             __builtin_amdgcn_s_waitcnt(0xF70);  // vmcnt(0): this tile's DMA has landed
             __syncthreads();
             __builtin_amdgcn_sched_barrier(0);
-            if (t + 1 < t1) {
-                issue((t + 1) * KT, pid, S[(t + 1) & 1]);
-                pid = page_of((t + 2) * KT);
+            const int mine = t + group;
+            if (mine + W < t1) {
+                issue((mine + W) * KT, pid, S[buffer(t + W)]);
+                pid = page_of((mine + 2 * W) * KT);
             }
             __builtin_amdgcn_sched_barrier(0);
-            if (live && t * KT < lim_hi) compute(t * KT, reinterpret_cast<const char*>(&S[t & 1]), edge);
+            if (live && (W == 1 || mine < t1) && mine * KT < lim_hi) compute(mine * KT, reinterpret_cast<const char*>(&S[buffer(t)]), edge);
         };
         int t = t0;
 #pragma unroll 1
-        for (; t < min(whole, t1); t++) step(t, std::false_type{});
+        for (; t + W <= min(whole, t1); t += W) step(t, std::false_type{});
 #pragma unroll 1
-        for (; t < t1; t++) step(t, std::true_type{});
+        for (; t < t1; t += W) step(t, std::true_type{});
     }
     l = lane_pair_sum<16>(l);
     l = lane_pair_sum<32>(l);
+    if constexpr (W == 2) {
+        static_assert(4 * 64 * (4 * KS + 2) * 4 <= (int)sizeof(S), "the second group's sums");
+        floatx4* room = reinterpret_cast<floatx4*>(S) + wave * 64 * KS;
+        float* ml = reinterpret_cast<float*>(S) + 4 * 64 * 4 * KS + wave * 128 + lane;
+        __syncthreads();  // the tiles are read
+        if (group) {
+#pragma unroll
+            for (int i = 0; i < KS; i++) room[i * 64 + lane] = acc[i];
+            ml[0] = m, ml[64] = l;
+        }
+        __syncthreads();
+        if (group) return;
+        const float mo = ml[0], mn = fmaxf(m, mo), ms = mn == -INFINITY ? 0.f : mn;
+        const float f = __builtin_amdgcn_exp2f((m - ms) * cs), fo = __builtin_amdgcn_exp2f((mo - ms) * cs);
+        m = mn;
+        l = fmaf(l, f, ml[64] * fo);
+#pragma unroll
+        for (int i = 0; i < KS; i++) {
+            const floatx4 z = room[i * 64 + lane];
+#pragma unroll
+            for (int e = 0; e < 4; e++) acc[i][e] = fmaf(acc[i][e], f, z[e] * fo);
+        }
+    }
     if (w0 + col >= rows) return;
     const int sees = sq.shown + qi;
     const float inv = sees > sq.len ? NAN : 1.0f / l;
     float* op = static_cast<float*>(a.out) + ((int64_t)(sq.first + qi) * a.hq + qh) * D;
-    float* rec = a.ws + ((int64_t)(pt.unit * pt.most + part) * 64 + wave * 16 + col) * (D + 4);
+    float* rec = a.ws + ((int64_t)(pt.unit * most + part) * 64 + wave * 16 + col) * (D + 4);
     if (parts > 1 && g == 0) *reinterpret_cast<floatx4*>(rec + D) = floatx4{m, l, cs, 0.f};
 #pragma unroll
     for (int i = 0; i < VN; i++)
@@ -1154,18 +1212,18 @@ __global__ __launch_bounds__(256, 2) void k_paged_prompt_f32(
 
 // Adds the parts of cut units, 16 rows to a workgroup: a launch, and one wait per eight parts.
 template <typename QT>
-__global__ __launch_bounds__(256) void k_prompt_join(const PagedAttn a, const int32_t* __restrict__ cu, const int32_t* __restrict__ lens, int shift, int keys) {
+__global__ __launch_bounds__(256) void k_prompt_join(const PagedAttn a, const int32_t* __restrict__ cu, const int32_t* __restrict__ lens, int shift, int keys, int most) {
     __shared__ __attribute__((aligned(16))) float room[256 * JOIN_ROOM];
     const PagedCache& c = a.c;
     const int G = a.G, per = 1 << (shift - 4), sub = blockIdx.x & (per - 1);
     Prompt pt;
-    if (!prompt_tile(c, cu, lens, G, shift, blockIdx.x / per, true, true, &pt)) return;
+    if (!prompt_tile(c, cu, lens, G, shift, blockIdx.x / per, most, true, &pt)) return;
     const int rows = pt.sq.n * G, r0 = (pt.tile << shift) + 16 * sub;
     if (r0 >= rows) return;
     const int last = limit_of(pt.sq, min((pt.tile << shift) + (1 << shift) - 1, rows - 1) / G);
-    const int parts = prompt_parts(pt.most, (last + keys - 1) / keys);
+    const int parts = prompt_parts(most, (last + keys - 1) / keys);
     if (parts == 1) return;
-    const uint32_t row = (c.D + 4) * 4, slot = row << shift, first = (uint32_t)(pt.unit * pt.most) * slot + 16 * sub * row;
+    const uint32_t row = (c.D + 4) * 4, slot = row << shift, first = (uint32_t)(pt.unit * most) * slot + 16 * sub * row;
     join_tile<QT, 0, 256>(a, pt.sq, pt.h, r0 >> 4, first, first, slot, parts, (uint32_t)SLOTS * slot, room);
 }
 
@@ -1217,11 +1275,14 @@ static int64_t units_of(int64_t batch, int64_t rows, int G, int hkv, int tile) {
 // 4 of 64: 8 x 16 rows over 1000 (288) 24 against 22, 256 rows over nothing (516) 13 against 19.
 static bool takes_prompt(int64_t batch, int64_t rows, int G, int hkv, int64_t capacity, bool kv16) {
     const int64_t tiles = units_of(batch, rows, G, hkv, 16);
-    return tiles >= 1024 || tiles * cdiv(capacity, 128) >= (kv16 ? 8192 : 2048);
+    return tiles >= 1024 || tiles * cdiv(capacity, 128) >= (kv16 ? 8192 : 1024);
 }
-// Whether their units are cut: where they alone, about half a tile per sequence short of the most
-// there can be, would leave CUs idle (256 rows over 16000, 64 units: 447 us whole, 146 cut;
-// 8 x 128 rows over nothing, 256 units: 17 whole, 22 cut).
+// Whether their units are few: where they alone, about half a tile per sequence short of the most
+// there can be, would leave CUs idle.  Then workgroups are twice as wide (f16 caches, head sizes up
+// to 128) and units are cut while there are CUs.  256 rows over 16000, 64 units: 447 us whole, 137
+// cut into eight, 150 into four with twice the wavefronts, 256 over 2000 43.7 and 41.6; one prompt of
+// 900 rows, 232 units: 38 cut in two, 23 with twice the wavefronts; 8 x 128 rows over nothing, 256
+// units: 17 whole, 22 cut.
 static bool cuts(int64_t batch, int64_t rows, int G, int hkv, int tile) { return hkv * (cdiv(rows * G, tile) + batch / 2) < 256; }
 
 // The records of the runs, or of cut prompts where the packed rows may be such, whatever the table.
@@ -1272,13 +1333,22 @@ template <typename KVT, typename QT, int DP>
 static int launch_prompt(const PagedAttn& a, hipStream_t s) {
     constexpr bool H16 = std::is_same_v<KVT, _Float16>;
     constexpr int ROWS = H16 ? 128 : 64, KEYS = H16 ? PromptTile<DP>::KT : 4096 / DP;
+    // Few units: two groups of wavefronts to a workgroup, and parts for the CUs that are left.
     const int64_t units = units_of(a.c.batch, a.c.rows, a.G, a.c.hkv, ROWS);
     const bool cut = cuts(a.c.batch, a.c.rows, a.G, a.c.hkv, ROWS);
-    const dim3 grid((unsigned)(cut ? SLOTS : units));
+    const int64_t likely = a.c.hkv * (cdiv(a.c.rows * (int64_t)a.G, ROWS) + a.c.batch / 2);  // (at least half of units)
+    constexpr int WIDE = H16 && DP > 128 ? 1 : 2;
+    const int most = !cut ? 1 : (int)std::max<int64_t>(WIDE == 2 ? SLOTS / 2 / likely : SLOTS / units, 1);
+    const dim3 grid((unsigned)(units * most));
     const char *kp = static_cast<const char*>(a.c.k), *vp = static_cast<const char*>(a.c.v);
-    if constexpr (H16) k_paged_prompt<QT, DP><<<grid, 256, 0, s>>>(a, a.c.table, a.c.cu, a.c.lens, kp, vp, cut);
-    else k_paged_prompt_f32<DP><<<grid, 256, 0, s>>>(a, a.c.table, a.c.cu, a.c.lens, kp, vp, cut);
-    if (cut) k_prompt_join<QT><<<dim3((unsigned)(units * (ROWS / 16))), 256, 0, s>>>(a, a.c.cu, a.c.lens, H16 ? 7 : 6, KEYS);
+    auto launch = [&](auto w) {
+        constexpr int W = decltype(w)::value;
+        if constexpr (H16) k_paged_prompt<QT, DP, W><<<grid, 256 * W, 0, s>>>(a, a.c.table, a.c.cu, a.c.lens, kp, vp, most);
+        else k_paged_prompt_f32<DP, W><<<grid, 256 * W, 0, s>>>(a, a.c.table, a.c.cu, a.c.lens, kp, vp, most);
+    };
+    if (cut) launch(std::integral_constant<int, WIDE>{});
+    else launch(std::integral_constant<int, 1>{});
+    if (most > 1) k_prompt_join<QT><<<dim3((unsigned)(units * (ROWS / 16))), 256, 0, s>>>(a, a.c.cu, a.c.lens, H16 ? 7 : 6, KEYS, most);
     hipError_t e = hipGetLastError();
     return e == hipSuccess ? TL_HIP_OK : hip_fail(e, "paged attention launch");
 }
