@@ -162,6 +162,9 @@ def test_prefill(dev, qt, kt, hkv, G, D, ps, new, past, extra):
     (1, 3, 256, 128, [200, 70], [333, 0], 0, 65536),
     (1, 5, 136, 16, [90], [400], 0, 65536),
     (1, 1, 40, 256, [300], [2000], 0, 65536),
+    (40, 4, 64, 16, [150, 10], [100, 0], 1, 0),          # fewer tiles than CUs, whole
+    (50, 4, 128, 64, [128], [300], 0, 0),
+    (9, 33, 72, 32, [31, 1, 60], [0, 64, 3], 2, 0),
     (64, 4, 64, 64, [135], [60], 0, 0),                  # enough tiles to stay whole
     (64, 4, 128, 16, [129, 2], [0, 33], 3, 0),
     (66, 4, 80, 64, [128], [0], 0, 0),

@@ -994,17 +994,17 @@ __global__ __launch_bounds__(256 * W, (DP > 128 ? 1 : 2)) void k_paged_prompt(
 // keys 4 g + e of 16; one 16-byte read of a value row feeds four matrix instructions, dimension
 // 64 j + 4 r + y in row r of number y.  3 prompts of 1100 rows together, 32 heads over 4 of 64: 38 us
 // (2.5 GFLOP, 66 TFLOP/s); while a CU works its matrix units do 59 % of the time.
-template <int DP, int W>  // W as above
-__global__ __launch_bounds__(256 * W, 2) void k_paged_prompt_f32(
+template <int DP>
+__global__ __launch_bounds__(256, 2) void k_paged_prompt_f32(
     const PagedAttn a, const int32_t* __restrict__ table, const int32_t* __restrict__ cu, const int32_t* __restrict__ lens,
     const char* __restrict__ kp, const char* __restrict__ vp, int most) {
     constexpr int CPR = DP / 4, KT = 1024 / CPR, U = 4, RPW = KT / 4, ST = KT / 16, KS = DP / 16, VN = DP / 64;
     struct Stage {
         uint4 k[KT * CPR], v[KT * CPR];
     };
-    __shared__ __attribute__((aligned(16))) Stage S[2 * W];
+    __shared__ __attribute__((aligned(16))) Stage S[2];
     const PagedCache& c = a.c;
-    const int lane = threadIdx.x & 63, wave4 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = wave4 & 3, group = W == 1 ? 0 : wave4 >> 2, col = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
     const int G = a.G, D = c.D, page = 1 << c.shift;
     Prompt pt;
     if (!prompt_tile(c, cu, lens, G, 6, blockIdx.x, most, false, &pt)) return;
@@ -1140,53 +1140,28 @@ __global__ __launch_bounds__(256 * W, 2) void k_paged_prompt_f32(
     };
 
     if (t0 < t1) {
-        auto buffer = [&](int t) { return W == 1 ? t & 1 : 2 * group + (((t - t0) >> 1) & 1); };
-        int pid = page_of((t0 + group) * KT);
-        if (W == 1 || t0 + group < t1) issue((t0 + group) * KT, pid, S[buffer(t0)]);
-        pid = page_of((t0 + W + group) * KT);
-        auto step = [&](int t, auto edge) __attribute__((always_inline)) {  // tiles t .. t + W - 1
+        int pid = page_of(t0 * KT);
+        issue(t0 * KT, pid, S[t0 & 1]);
+        pid = page_of((t0 + 1) * KT);
+        auto step = [&](int t, auto edge) __attribute__((always_inline)) {
             __builtin_amdgcn_s_waitcnt(0xF70);  // vmcnt(0): this tile's DMA has landed
             __syncthreads();
             __builtin_amdgcn_sched_barrier(0);
-            const int mine = t + group;
-            if (mine + W < t1) {
-                issue((mine + W) * KT, pid, S[buffer(t + W)]);
-                pid = page_of((mine + 2 * W) * KT);
+            if (t + 1 < t1) {
+                issue((t + 1) * KT, pid, S[(t + 1) & 1]);
+                pid = page_of((t + 2) * KT);
             }
             __builtin_amdgcn_sched_barrier(0);
-            if (live && (W == 1 || mine < t1) && mine * KT < lim_hi) compute(mine * KT, reinterpret_cast<const char*>(&S[buffer(t)]), edge);
+            if (live && t * KT < lim_hi) compute(t * KT, reinterpret_cast<const char*>(&S[t & 1]), edge);
         };
         int t = t0;
 #pragma unroll 1
-        for (; t + W <= min(whole, t1); t += W) step(t, std::false_type{});
+        for (; t < min(whole, t1); t++) step(t, std::false_type{});
 #pragma unroll 1
-        for (; t < t1; t += W) step(t, std::true_type{});
+        for (; t < t1; t++) step(t, std::true_type{});
     }
     l = lane_pair_sum<16>(l);
     l = lane_pair_sum<32>(l);
-    if constexpr (W == 2) {
-        static_assert(4 * 64 * (4 * KS + 2) * 4 <= (int)sizeof(S), "the second group's sums");
-        floatx4* room = reinterpret_cast<floatx4*>(S) + wave * 64 * KS;
-        float* ml = reinterpret_cast<float*>(S) + 4 * 64 * 4 * KS + wave * 128 + lane;
-        __syncthreads();  // the tiles are read
-        if (group) {
-#pragma unroll
-            for (int i = 0; i < KS; i++) room[i * 64 + lane] = acc[i];
-            ml[0] = m, ml[64] = l;
-        }
-        __syncthreads();
-        if (group) return;
-        const float mo = ml[0], mn = fmaxf(m, mo), ms = mn == -INFINITY ? 0.f : mn;
-        const float f = __builtin_amdgcn_exp2f((m - ms) * cs), fo = __builtin_amdgcn_exp2f((mo - ms) * cs);
-        m = mn;
-        l = fmaf(l, f, ml[64] * fo);
-#pragma unroll
-        for (int i = 0; i < KS; i++) {
-            const floatx4 z = room[i * 64 + lane];
-#pragma unroll
-            for (int e = 0; e < 4; e++) acc[i][e] = fmaf(acc[i][e], f, z[e] * fo);
-        }
-    }
     if (w0 + col >= rows) return;
     const int sees = sq.shown + qi;
     const float inv = sees > sq.len ? NAN : 1.0f / l;
@@ -1275,11 +1250,11 @@ static int64_t units_of(int64_t batch, int64_t rows, int G, int hkv, int tile) {
 // 4 of 64: 8 x 16 rows over 1000 (288) 24 against 22, 256 rows over nothing (516) 13 against 19.
 static bool takes_prompt(int64_t batch, int64_t rows, int G, int hkv, int64_t capacity, bool kv16) {
     const int64_t tiles = units_of(batch, rows, G, hkv, 16);
-    return tiles >= 1024 || tiles * cdiv(capacity, 128) >= (kv16 ? 8192 : 1024);
+    return tiles >= 1024 || tiles * cdiv(capacity, 128) >= (kv16 ? 8192 : 2048);
 }
 // Whether their units are few: where they alone, about half a tile per sequence short of the most
 // there can be, would leave CUs idle.  Then workgroups are twice as wide (f16 caches, head sizes up
-// to 128) and units are cut while there are CUs.  256 rows over 16000, 64 units: 447 us whole, 137
+// to 128) and units are cut while there are CUs.  256 rows over 16000, 64 units: 447 us whole, 145
 // cut into eight, 150 into four with twice the wavefronts, 256 over 2000 43.7 and 41.6; one prompt of
 // 900 rows, 232 units: 38 cut in two, 23 with twice the wavefronts; 8 x 128 rows over nothing, 256
 // units: 17 whole, 22 cut.
@@ -1337,17 +1312,17 @@ static int launch_prompt(const PagedAttn& a, hipStream_t s) {
     const int64_t units = units_of(a.c.batch, a.c.rows, a.G, a.c.hkv, ROWS);
     const bool cut = cuts(a.c.batch, a.c.rows, a.G, a.c.hkv, ROWS);
     const int64_t likely = a.c.hkv * (cdiv(a.c.rows * (int64_t)a.G, ROWS) + a.c.batch / 2);  // (at least half of units)
-    constexpr int WIDE = H16 && DP > 128 ? 1 : 2;
-    const int most = !cut ? 1 : (int)std::max<int64_t>(WIDE == 2 ? SLOTS / 2 / likely : SLOTS / units, 1);
+    const int most = !cut ? 1 : (int)std::max<int64_t>(H16 && DP <= 128 ? SLOTS / 2 / likely : SLOTS / units, 1);
     const dim3 grid((unsigned)(units * most));
     const char *kp = static_cast<const char*>(a.c.k), *vp = static_cast<const char*>(a.c.v);
-    auto launch = [&](auto w) {
-        constexpr int W = decltype(w)::value;
-        if constexpr (H16) k_paged_prompt<QT, DP, W><<<grid, 256 * W, 0, s>>>(a, a.c.table, a.c.cu, a.c.lens, kp, vp, most);
-        else k_paged_prompt_f32<DP, W><<<grid, 256 * W, 0, s>>>(a, a.c.table, a.c.cu, a.c.lens, kp, vp, most);
-    };
-    if (cut) launch(std::integral_constant<int, WIDE>{});
-    else launch(std::integral_constant<int, 1>{});
+    if constexpr (H16 && DP <= 128) {
+        if (cut) k_paged_prompt<QT, DP, 2><<<grid, 512, 0, s>>>(a, a.c.table, a.c.cu, a.c.lens, kp, vp, most);
+        else k_paged_prompt<QT, DP, 1><<<grid, 256, 0, s>>>(a, a.c.table, a.c.cu, a.c.lens, kp, vp, most);
+    } else if constexpr (H16) {
+        k_paged_prompt<QT, DP, 1><<<grid, 256, 0, s>>>(a, a.c.table, a.c.cu, a.c.lens, kp, vp, most);
+    } else {
+        k_paged_prompt_f32<DP><<<grid, 256, 0, s>>>(a, a.c.table, a.c.cu, a.c.lens, kp, vp, most);
+    }
     if (most > 1) k_prompt_join<QT><<<dim3((unsigned)(units * (ROWS / 16))), 256, 0, s>>>(a, a.c.cu, a.c.lens, H16 ? 7 : 6, KEYS, most);
     hipError_t e = hipGetLastError();
     return e == hipSuccess ? TL_HIP_OK : hip_fail(e, "paged attention launch");
